@@ -48,10 +48,15 @@ enum momij_status {
     MOMIJ_ERR_CUDA = 7,              /* a CUDA runtime call failed */
     MOMIJ_ERR_NCCL = 8,              /* an NCCL call failed (expert parallel) */
     MOMIJ_ERR_TIMEOUT = 9,           /* a bounded device-side wait gave up */
-    MOMIJ_ERR_STOPPED = 10           /* the stop flag was set */
+    MOMIJ_ERR_STOPPED = 10,          /* the stop flag was set */
+    MOMIJ_ERR_PAGE = 11              /* a cache page, length or position out of range (device-detected) */
 };
 
-enum momij_dtype { MOMIJ_DTYPE_BF16 = 0, MOMIJ_DTYPE_F16 = 1 };
+enum momij_dtype {
+    MOMIJ_DTYPE_BF16 = 0,
+    MOMIJ_DTYPE_F16 = 1,
+    MOMIJ_DTYPE_F32 = 2 /* logits of momij_process_logits only */
+};
 
 #define MOMIJ_MAX_PAIRS 1024
 /* momij_moe_expert_ffn / momij_moe_forward: M*Ktop up to this many pairs
@@ -248,6 +253,98 @@ int momij_moe_block(void* h, const void* norm_w, float eps, const void* w_gate, 
                     const void* s_dn, const void* b_dn, int32_t* inds, float* scores, int M, int H,
                     int I, int E, int Ktop, int gs, float clamp, int dtype, void* workspace,
                     size_t workspace_bytes, momij_stream_t stream);
+
+/* ---- attention over an 8-bit paged cache, 4-bit projections, logits ----------
+ *
+ * Cache (caller-owned, aliased): pages of MOMIJ_KV_PAGE = 64 consecutive tokens,
+ *   k_codes uint8 [n_pages, Hkv, 64, D]   v_codes uint8 [n_pages, Hkv, D, 64]
+ *   k_scales, v_scales fp32 [n_pages, Hkv]
+ * A code c stands for (c - 128) * scale of its page and head (c in 1..255; a
+ * scale is 0, NaN or between 2^-64 and 2^100).  block_table int32 [B,
+ * table_cols]: the page of tokens 64 i .. 64 i + 63 of sequence b.  lens int32
+ * [B]: tokens of each sequence in the cache, INCLUDING the ones that a call
+ * appends or queries.  cu_q int32 [B + 1]: row offsets of each sequence's new
+ * tokens in qkv / q, or NULL for T / B each; max_q: the most of them in one
+ * sequence (0: unknown, up to T).  lens, cu_q and block_table are read on the
+ * device; a page, length or row outside its range is skipped and reported as
+ * MOMIJ_ERR_PAGE by momij_moe_synchronize(stream, workspace).  D is 64 or 128,
+ * Hq a multiple of Hkv.  Codes and the rotation table start on 16-byte
+ * boundaries, 16-bit rows on 8-byte boundaries (attention's q: any).
+ */
+#define MOMIJ_KV_PAGE 64
+
+/* Head norms, rotation and append in one launch.  Row t of qkv (ld elements
+ * apart, ld % 4 == 0) holds Hq query, Hkv key and Hkv value heads of D:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight          (queries, keys; weight [D], NULL: no norm)
+ *   the first rot elements of y turn by the angles of the token's position
+ *   (rope fp32 [rope_rows, rot]: rot/2 cosines, then rot/2 sines; pairs
+ *   (i, i + rot/2), or (2i, 2i + 1) if interleaved; rot % 8 == 0, 0: none)
+ * q_out [T, Hq, D] gets the queries; keys and values become codes at positions
+ * lens[b] - n_b .. lens[b] - 1.  A page's scale is amax / 127 over its tokens so
+ * far; when new tokens raise it, the page's earlier tokens are recoded (rounded
+ * once more).  A page that receives an infinity or NaN gets a NaN scale and
+ * reads as NaN until its first row is written again.  Pages must not be shared
+ * by sequences that append to them.  workspace may be NULL (no error report).
+ * Replaces: the query/key norm with rotation (MapleFused.swift:260-325) and the
+ * cache write (SeedlessMetal.swift:2794-3004; 16-bit there). */
+int momij_qk_norm_rope_append(const void* qkv, long long ld, void* q_out, const void* q_weight, const void* k_weight,
+                              float eps, const float* rope, int rope_rows, int rot, int interleaved, uint8_t* k_codes,
+                              uint8_t* v_codes, float* k_scales, float* v_scales, int n_pages,
+                              const int32_t* block_table, int table_cols, const int32_t* lens, const int32_t* cu_q,
+                              int T, int B, int max_q, int Hq, int Hkv, int D, int dtype, void* workspace,
+                              size_t workspace_bytes, momij_stream_t stream);
+
+/* Cache values of `count` tokens per sequence from first[b] on (NULL: 0), as
+ * k_out, v_out [B, count, Hkv, D]; tokens at or past lens[b] give zeros. */
+int momij_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_scales, const float* v_scales,
+                     int n_pages, const int32_t* block_table, int table_cols, const int32_t* lens,
+                     const int32_t* first, int count, void* k_out, void* v_out, int B, int Hkv, int D, int dtype,
+                     void* workspace, size_t workspace_bytes, momij_stream_t stream);
+
+/* Workspace bytes of momij_attention for T query tokens of Hq heads; zero-filled
+ * once before its first use, reusable for any call of up to that size (its words
+ * are also what the append and the read report errors in: 256 bytes). */
+size_t momij_attention_workspace_size(int T, int Hq);
+
+/* out[t, hq] = sum_j softmax_j(scale * q[t, hq] . k_j) v_j over the cached
+ * positions p - window < j <= p of the token's sequence (window 0: all), with
+ * p = lens[b] - n_b + i for its i-th new token; kv head hq / (Hq / Hkv).  A row
+ * that sees no position (lens[b] < n_b) gives zeros.  Rows of q and out are ldq
+ * and ldo elements apart (ldo % 4 == 0).  One launch; the result does not depend
+ * on scheduling.
+ * Replaces: the 16-bit attention of SeedlessMetal.swift:2794-3004. */
+int momij_attention(const void* q, long long ldq, void* out, long long ldo, const uint8_t* k_codes,
+                    const uint8_t* v_codes, const float* k_scales, const float* v_scales, int n_pages,
+                    const int32_t* block_table, int table_cols, const int32_t* lens, const int32_t* cu_q, int T, int B,
+                    int max_q, int Hq, int Hkv, int D, float scale, int window, int dtype, void* workspace,
+                    size_t workspace_bytes, momij_stream_t stream);
+
+/* y[m, n] = sum_k (s[n, k/gs] * q[n, k] + b[n, k/gs]) * x[m, k] with 4-bit codes
+ * (MLX affine, transpose=true): w uint32 [N, K/8], code k at bits [4(k%8),
+ * 4(k%8)+3]; s, b 16-bit [N, K/gs], gs 64 or 128, K % gs == 0; w 8-byte aligned.
+ * Rows of x and y are ldx and ldy elements apart.  For few tokens: up to 32 share
+ * a pass over the matrix (fewer for K above 3,000 or so).
+ * Replaces: the 4-bit output head's product (SeedlessMetal.swift:2598-2716) and
+ * MLX.quantizedMM of 4-bit projections (QuantProj.swift). */
+int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const void* scales, const void* biases, void* y,
+               long long ldy, int M, int K, int N, int gs, int dtype, momij_stream_t stream);
+
+/* Penalties, biases and grammar mask on logits [B, V] (rows ld elements apart;
+ * dtype MOMIJ_DTYPE_BF16, _F16 or _F32) -> out fp32 [B, V], for each token with c
+ * occurrences in its row's history:
+ *   c > 0: l = l > 0 ? l / repetition[b] : l * repetition[b]
+ *   l = l - (frequency[b] * c + presence[b] * [c > 0]);  l = l + bias
+ *   l = -inf where bit v % 32 of allowed[b * ld_allowed + v / 32] is 0
+ * history int32 [n_history], row b's ids at cu_history[b] .. cu_history[b+1]-1;
+ * bias_ids and bias [n_bias] by cu_bias alike, the last entry of a token holds;
+ * ids outside [0, V) are skipped.  Any of the inputs may be NULL (no history,
+ * repetition 1, presence and frequency 0, no bias, no mask).
+ * Replaces: LogitsProcessor.swift's penalties and XGrammarGuide.swift's mask. */
+int momij_process_logits(const void* logits, long long ld, int dtype, float* out, int B, int V,
+                         const int32_t* history, const int32_t* cu_history, int n_history, const float* repetition,
+                         const float* presence, const float* frequency, const int32_t* bias_ids, const float* bias,
+                         const int32_t* cu_bias, int n_bias, const uint32_t* allowed, long long ld_allowed,
+                         momij_stream_t stream);
 
 /* Expert-parallel decode (experts sharded contiguously: rank r owns experts
  * [r*E/world, (r+1)*E/world)).  The caller runs the two all-to-all exchanges

@@ -20,6 +20,7 @@
 #include "layer.cuh"
 #include "token.cuh"
 #include "prefill.cuh"
+#include "host.cuh"
 
 using namespace momij;
 
@@ -1155,6 +1156,16 @@ int ffn_after_plan(const void* x, const uint32_t* w_ug, const void* s_ug, const 
 
 }  // namespace
 
+// What the entry points outside this file share (host.cuh).
+namespace momij {
+int host_check_device() { return check_device(); }
+int host_sm_count() { return current_device_sm_count(); }
+bool host_pdl() { return pdl_enabled(); }
+const int32_t* host_stop_flag() { return g_stop_flag.load(); }
+int host_spin_limit() { return spin_limit(); }
+void* host_tensor_map_encoder() { return reinterpret_cast<void*>(tensor_map_encoder()); }
+}  // namespace momij
+
 extern "C" {
 
 const char* momij_status_string(int status) {
@@ -1170,6 +1181,7 @@ const char* momij_status_string(int status) {
         case MOMIJ_ERR_NCCL: return "NCCL error";
         case MOMIJ_ERR_TIMEOUT: return "device-side wait timed out";
         case MOMIJ_ERR_STOPPED: return "stopped";
+        case MOMIJ_ERR_PAGE: return "cache page or position out of range";
         default: return "unknown status";
     }
 }

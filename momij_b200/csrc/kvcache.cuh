@@ -1,0 +1,37 @@
+// kvcache.cuh -- the 8-bit paged key/value cache shared by its writer
+// (kvcache.cu) and the attention that reads it (attn.cu, attn_prefill.cu).
+//
+//   K codes   uint8 [pages, Hkv, 64, D]   V codes  uint8 [pages, Hkv, D, 64]
+//   K scales  fp32  [pages, Hkv]          V scales fp32  [pages, Hkv]
+// A code c in 1..255 stands for (c - 128) * scale of its page and head.  A
+// page holds 64 consecutive tokens of one sequence; block_table[b, i] names
+// the page of tokens 64 i .. 64 i + 63 of sequence b.
+//   * offset codes: (c ^ 0x64 << 8) is the fp16 number 1024 + c, so a byte
+//     permute and one subtraction of 1152 make two operands of the matrix
+//     units from two codes, without a sign fix;
+//   * V transposed: the product with the weights sums over tokens, which then
+//     lie side by side like the dimensions of K do for the scores.
+#pragma once
+
+#include "common.cuh"
+
+namespace momij {
+
+constexpr int kPage = 64;
+
+// Control words at the start of an attention workspace; [1] and [2] are the
+// words momij_moe_synchronize reads ([1] of the latest call, [2] sticky).
+enum { kAttnStatus = 1, kAttnError = 2, kAttnHeader = 256 };  // (the header's size in bytes)
+
+__device__ __forceinline__ void cache_error(int32_t* ws, int code) {
+    if (ws) atomicMax(ws + kAttnError, code);
+}
+
+// Two codes (bytes `sel` of w) as packed fp16 integers -127 .. 127.
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t w, uint32_t sel) {
+    uint32_t h = __byte_perm(w, 0x64646464u, sel), r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));  // 1152
+    return r;
+}
+
+}  // namespace momij
