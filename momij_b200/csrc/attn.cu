@@ -17,16 +17,22 @@
 // power of two, which holds bf16's 8 bits exactly.
 //
 // Work.  A cache read once is all that a decode step needs, so the heads of a
-// group and the drafted tokens share it: a row block is up to 16 or 32 (token,
+// group and the drafted tokens share it: a row block is 8, 16 or 32 (token,
 // head) rows of one sequence and one kv head, multiplied by mma.sync m16n8k16
-// (rows in M; tcgen05's 128 rows would be mostly empty).  The (row block, head,
-// page) triples of all sequences form one line that is cut into equal shares,
-// one per block, so that ragged batches load every SM alike; a block's eight
-// warps take half pages in turn, each through its own ring of cp.async stages
-// (no barrier in the loop), and join their results at the end.  A segment
-// that several blocks share leaves partial results in the workspace; the block
-// that arrives last adds them in order (the result does not depend on which
-// one that is).
+// with the cache's codes as the 16-row operand (tokens for the scores,
+// dimensions for the outputs) and the rows as its 8 columns: a decode step's
+// few rows waste little, every code is converted once, and the outputs take
+// 32 registers per 8 rows (tcgen05's 128 rows would be mostly empty).  The
+// weights turn from the first product's result into the second's operand by
+// an 8x8 transposition between lanes (movmatrix).
+//
+// The (row block, head, page) triples of all sequences form one line that is
+// cut into equal shares, one per block, so that ragged batches load every SM
+// alike; a block's warps take half pages in turn, each through its own ring of
+// cp.async stages (no barrier in the loop), and join their results at the end.
+// A segment that several blocks share leaves partial results in the workspace;
+// the block that arrives last adds them in order (the result does not depend
+// on which one that is).
 #include <algorithm>
 
 #include "attn.cuh"
@@ -35,21 +41,26 @@
 namespace momij {
 namespace {
 
-constexpr int kThreads = 256, kWarps = 8;
-constexpr int kStages = 3;
 constexpr int kMaxSeg = 4096;   // row blocks per launch (their prefix sums live in shared memory)
-constexpr int kMinPages = 4;    // pages per block at least: a half page for each warp
+constexpr int kMinPages = 4;    // pages per block at least, unless the segments are shorter
 constexpr int kMaxRows = 32;    // rows of a row block at most
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// Transposes an 8x8 matrix of 16-bit values held as row g, columns 2c, 2c + 1.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 
@@ -71,24 +82,31 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const AttnSeq& s, int
     return p;
 }
 
-template <int DT, int D, int MT>
-__global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
-    constexpr int RB = 16 * MT, KS = D / 16, NT = D / 8;
+template <int NB>
+struct Shape {  // of a block: warps and stages of their rings, by rows per block (8 NB)
+    static constexpr int kWarps = NB == 4 ? 8 : 12;
+    static constexpr int kStages = NB == 4 ? 3 : 2;
+};
+
+template <int DT, int D, int NB>
+__global__ void __launch_bounds__(Shape<NB>::kWarps * 32, 1) attn_kernel(const AttnArgs a) {
+    constexpr int kWarps = Shape<NB>::kWarps, kThreads = kWarps * 32, kStages = Shape<NB>::kStages;
+    constexpr int RB = 8 * NB, KS = D / 16, MD = D / 16;
     constexpr int kKBytes = 32 * D, kStage = 2 * kKBytes;  // a half page of K and of V
     constexpr int kOPitch = D + 4;
+    constexpr bool kSharedQ = NB == 4;  // q fragments in shared memory rather than registers
     extern __shared__ __align__(16) unsigned char smem[];
-    // [stages of all warps | joined results] [q fragments] [row factors, warp maxima and sums] [prefix]
-    unsigned char* s_stage = smem;
+    // [stages of all warps, then their results] [q fragments, row factors] [warp maxima and sums] [prefix]
     float* s_o = reinterpret_cast<float*>(smem);
     constexpr int kRing = kWarps * kStages * kStage;
     constexpr int kJoin = kWarps * RB * kOPitch * 4;
     constexpr int kArea = kRing > kJoin ? kRing : kJoin;
-    uint4* s_q = reinterpret_cast<uint4*>(smem + kArea);
-    float* s_fac = reinterpret_cast<float*>(smem + kArea + KS * MT * 512);
+    uint2* s_q = reinterpret_cast<uint2*>(smem + kArea);
+    float* s_fac = reinterpret_cast<float*>(smem + kArea + (kSharedQ ? KS * NB * 256 : 0));
     float* s_m = s_fac + RB;
     float* s_l = s_m + kWarps * RB;
     int* s_pref = reinterpret_cast<int*>(s_l + kWarps * RB);
-    __shared__ int s_scan[kWarps];
+    __shared__ int s_scan[kWarps], s_full[kWarps];
     __shared__ int s_last;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
@@ -97,17 +115,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
     if (tid == 0 && blockIdx.x == 0) a.ws[kAttnStatus] = stopped ? MOMIJ_ERR_STOPPED : MOMIJ_OK;
     if (stopped) return;
 
-    // ---- prefix sums of the segments' pages -----------------------------------
+    // ---- prefix sums of the segments' pages, and the segments that have any ---
     const int nseg = a.nb * a.nrb, per = (nseg + kThreads - 1) / kThreads;
-    int sum = 0;
+    int sum = 0, full = 0;
     for (int i = 0; i < per; ++i) {
         const int sg = tid * per + i;
         if (sg < nseg) {
-            const int b = a.b0 + sg / a.nrb;
-            const AttnSeq s = attn_sequence(a, b);
+            const AttnSeq s = attn_sequence(a, a.b0 + sg / a.nrb);
             const Span p = span_of(a, s, sg % a.nrb, RB);
             if (!s.ok && sg % a.nrb == 0) cache_error(a.ws, MOMIJ_ERR_PAGE);
             sum += p.hi - p.lo;
+            full += p.hi > p.lo;
             s_pref[sg + 1] = sum;  // within this thread's run
         }
     }
@@ -117,66 +135,89 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
         const int v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
     }
-    if (lane == 31) s_scan[warp] = inc;
+    full = __reduce_add_sync(0xffffffffu, full);
+    if (lane == 31) {
+        s_scan[warp] = inc;
+        s_full[warp] = full;
+    }
     __syncthreads();
-    int base = inc - sum;
-    for (int w = 0; w < warp; ++w) base += s_scan[w];
+    int base = inc - sum, total = 0, nfull = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) base += s_scan[w];
+        total += s_scan[w];
+        nfull += s_full[w];
+    }
     for (int i = 0; i < per; ++i) {
         const int sg = tid * per + i;
         if (sg < nseg) s_pref[sg + 1] += base;
     }
     if (tid == 0) s_pref[0] = 0;
     __syncthreads();
-    const long long U = (long long)s_pref[nseg] * a.Hkv;
+    const int U = total * a.Hkv;  // below 2^31: the host bounds the launch
 
     // rows that see no key at all
-    for (int sg = blockIdx.x; sg < nseg; sg += gridDim.x)
-        if (s_pref[sg + 1] == s_pref[sg]) {
-            const AttnSeq s = attn_sequence(a, a.b0 + sg / a.nrb);
-            const Span p = span_of(a, s, sg % a.nrb, RB);
-            for (int i = tid; i < p.rows * a.Hkv * D; i += kThreads) {
-                const int d = i % D, h = i / D % a.Hkv, r = i / D / a.Hkv + (sg % a.nrb) * RB;
-                a.out[(s.t0 + r / a.G) * a.ldo + (h * a.G + r % a.G) * D + d] = 0;
+    if (nfull < nseg)
+        for (int sg = blockIdx.x; sg < nseg; sg += gridDim.x)
+            if (s_pref[sg + 1] == s_pref[sg]) {
+                const AttnSeq s = attn_sequence(a, a.b0 + sg / a.nrb);
+                const Span p = span_of(a, s, sg % a.nrb, RB);
+                for (int i = tid; i < p.rows * a.Hkv * D; i += kThreads) {
+                    const int d = i % D, h = i / D % a.Hkv, r = i / D / a.Hkv + (sg % a.nrb) * RB;
+                    a.out[(s.t0 + r / a.G) * a.ldo + (h * a.G + r % a.G) * D + d] = 0;
+                }
             }
-        }
 
-    const long long want = (U + kMinPages - 1) / kMinPages;
-    const int nblk = (int)(want < gridDim.x ? want : gridDim.x);
+    // Blocks in use: all of them when there is a share of kMinPages for each,
+    // fewer for short contexts, but one per (segment, head) where those are
+    // shorter still: they are independent, and a block takes one at a time.
+    const int nblk = min((int)gridDim.x, max((U + kMinPages - 1) / kMinPages, min(nfull, 1 << 20) * a.Hkv));
     if ((int)blockIdx.x >= nblk) {
         pdl_launch_dependents();
         return;
     }
-    auto share = [&](int i) -> long long { return U * i / nblk; };
-    const long long u0 = share(blockIdx.x), u1 = share(blockIdx.x + 1);
+    const int sh_q = U / nblk, sh_r = U - sh_q * nblk;  // the first sh_r shares hold one unit more
+    auto share = [&](int i) -> int { return sh_q * i + min(i, sh_r); };
+    auto owner = [&](int x) -> int {
+        const int cut = sh_r * (sh_q + 1);
+        return x < cut ? x / (sh_q + 1) : sh_r + (x - cut) / sh_q;
+    };
+    const int u0 = share(blockIdx.x), u1 = share(blockIdx.x + 1);
 
-    long long u = u0;
+    int u = u0;
     int seg = 0;
     {  // the segment that holds u0
         int lo = 0, hi = nseg - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if ((long long)s_pref[mid] * a.Hkv <= u) lo = mid;
+            if (s_pref[mid] * a.Hkv <= u) lo = mid;
             else hi = mid - 1;
         }
         seg = lo;
     }
     while (u < u1) {
-        while ((long long)s_pref[seg + 1] * a.Hkv <= u) ++seg;
-        const int b = a.b0 + seg / a.nrb, rb = seg % a.nrb;
+        while (s_pref[seg + 1] * a.Hkv <= u) ++seg;
+        const int b = a.b0 + seg / a.nrb, row0 = (seg % a.nrb) * RB;
         const AttnSeq sq = attn_sequence(a, b);
-        const Span span = span_of(a, sq, rb, RB);
+        const Span span = span_of(a, sq, seg % a.nrb, RB);
         const int np = span.hi - span.lo;
-        const long long sbase = (long long)s_pref[seg] * a.Hkv;
-        const int h = (int)((u - sbase) / np);
-        const long long hb = sbase + (long long)h * np;  // first unit of this (segment, head)
-        const int pa = (int)(u - hb), pb = (int)min((long long)np, u1 - hb);
-        const int row0 = rb * RB;
+        const int sbase = s_pref[seg] * a.Hkv;
+        const int h = (u - sbase) / np;
+        const int hb = sbase + h * np;  // first unit of this (segment, head)
+        const int pa = u - hb, pb = min(np, u1 - hb);
 
-        // ---- this warp's half pages, three stages ahead ------------------------
+        // ---- this warp's half pages -------------------------------------------
         const int n_items = 2 * (pb - pa);
         const int keys_hi = sq.past + (row0 + span.rows - 1) / a.G + 1;
         const int keys_lo = a.window > 0 ? max(0, sq.past + row0 / a.G - a.window + 1) : 0;
-        unsigned char* ring = s_stage + warp * (kStages * kStage);
+        unsigned char* ring = smem + warp * (kStages * kStage);
+        const uint32_t ring32 = smem_u32(ring);
+        // A lane's 16 bytes of a copy of 512: K rows of 128 bytes swap their
+        // halves when odd, so that two rows read together cover all banks.
+        const uint32_t kdst = D == 128 ? (lane >> 3) * 128 + (((lane & 7) ^ (((lane >> 3) & 1) << 2)) << 4) : lane * 16;
+        const uint8_t* kbase = a.k + (long long)h * (kPage * D) + lane * 16;
+        const uint8_t* vbase = a.v + (long long)h * (kPage * D) + (lane >> 1) * kPage + (lane & 1) * 16;
+        const int32_t* trow = a.table + (long long)b * a.table_cols + span.lo + pa;
         // Returns the page's scales, which the caller keeps until the stage's turn
         // (read past L1: the append before this call may still have been
         // running when this block started).
@@ -184,207 +225,233 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
             float2 sc = make_float2(0.f, 0.f);
             const int item = warp + kWarps * it;
             if (item < n_items) {
-                const int pg = span.lo + pa + (item >> 1), half = item & 1;
-                const int t0 = pg * kPage + half * 32;
+                const int t0 = (span.lo + pa) * kPage + item * 32;
                 if (t0 < keys_hi && t0 + 32 > keys_lo) {
-                    int page = __ldg(a.table + (long long)b * a.table_cols + pg);
-                    const bool in = page >= 0 && page < a.n_pages;
+                    int page = __ldg(trow + (item >> 1));
+                    const bool in = (unsigned)page < (unsigned)a.n_pages;
                     if (!in) {
                         if (lane == 0) cache_error(a.ws, MOMIJ_ERR_PAGE);
                         page = 0;
                     }
-                    const long long ph = (long long)page * a.Hkv + h;
-                    const uint8_t* kp = a.k + ph * (kPage * D) + half * kKBytes;
-                    const uint8_t* vp = a.v + ph * (kPage * D) + half * 32;
-                    const uint32_t dst = smem_u32(ring + slot * kStage);
+                    const long long ph = (long long)page * a.Hkv;
+                    const uint8_t* kp = kbase + ph * (kPage * D) + (item & 1) * kKBytes;
+                    const uint8_t* vp = vbase + ph * (kPage * D) + (item & 1) * 32;
+                    const uint32_t dst = ring32 + slot * kStage;
 #pragma unroll
-                    for (int i = 0; i < kKBytes / 512; ++i) {
-                        const int ci = i * 32 + lane, row = ci / (D / 16), ch = ci % (D / 16);
-                        // 128-byte rows: odd rows swap their halves, so that two rows cover all banks
-                        const int sw = D == 128 ? ch ^ ((row & 1) << 2) : ch;
-                        cp_async16(dst + row * D + sw * 16, kp + ci * 16, in);
-                    }
+                    for (int i = 0; i < kKBytes / 512; ++i) cp_async16(dst + kdst + i * 512, kp + i * 512, in);
 #pragma unroll
-                    for (int i = 0; i < kKBytes / 512; ++i) {
-                        const int ci = i * 32 + lane;
-                        cp_async16(dst + kKBytes + ci * 16, vp + (ci >> 1) * kPage + (ci & 1) * 16, in);
-                    }
-                    sc.x = in ? __ldcg(a.ks + ph) : NAN;  // a bad page shows in the output too
-                    sc.y = in ? __ldcg(a.vs + ph) : NAN;
+                    for (int i = 0; i < kKBytes / 512; ++i)
+                        cp_async16(dst + kKBytes + lane * 16 + i * 512, vp + i * (16 * kPage), in);
+                    sc.x = in ? __ldcg(a.ks + ph + h) : NAN;  // a bad page shows in the output too
+                    sc.y = in ? __ldcg(a.vs + ph + h) : NAN;
                 }
             }
             cp_async_commit();
             return sc;
         };
-        float2 sc0 = issue(0, 0), sc1 = issue(1, 1);
+        float2 sc[kStages - 1];
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) sc[i] = issue(i, i);
 
-        // ---- q of the row block as fp16 fragments ------------------------------
-        for (int r = warp; r < RB; r += kWarps) {
-            constexpr int EPL = D / 32;  // elements a lane holds
-            float f[EPL];
+        // ---- q as fp16 fragments: lane (g, c) holds, for row g of each 8, the
+        // 16 elements from 64 i + 16 c on ------------------------------------------
+        uint32_t qf[kSharedQ ? 1 : NB][KS][2];
+        float fac[NB][2];
+        auto load_q = [&](int nb, uint32_t (&f)[KS][2]) -> float {
+            const int r = 8 * nb + g, row = row0 + r;
+            float e[D / 64][16];
             uint32_t top = 0;
-            const int row = row0 + r;
+            const uint16_t* src = a.q + (sq.t0 + row / a.G) * a.ldq + (h * a.G + row % a.G) * D + 16 * c;
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) f[e] = 0.f;
-            if (r < span.rows) {
-                const uint16_t* src = a.q + (sq.t0 + row / a.G) * a.ldq + (h * a.G + row % a.G) * D + lane * EPL;
+            for (int i = 0; i < D / 64; ++i) {
+                uint32_t w[8];
 #pragma unroll
-                for (int e = 0; e < EPL; ++e) {
-                    f[e] = Half<DT>::to_f(__ldg(src + e));
-                    top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+                for (int k = 0; k < 8; ++k) w[k] = 0;
+                if (r < span.rows) {
+                    if (a.qvec) {
+                        *reinterpret_cast<uint4*>(w) = __ldg(reinterpret_cast<const uint4*>(src + 64 * i));
+                        *reinterpret_cast<uint4*>(w + 4) = __ldg(reinterpret_cast<const uint4*>(src + 64 * i) + 1);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            w[k] = __ldg(src + 64 * i + 2 * k) | ((uint32_t)__ldg(src + 64 * i + 2 * k + 1) << 16);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    e[i][2 * k] = Half<DT>::to_f((uint16_t)(w[k] & 0xffffu));
+                    e[i][2 * k + 1] = Half<DT>::to_f((uint16_t)(w[k] >> 16));
+                    top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
                 }
             }
-            top = __reduce_max_sync(0xffffffffu, top);
-            int sh = 0;  // the row's largest magnitude becomes 2^13 .. 2^14 (zeros, infinities and NaN: left)
-            if (top != 0 && top < 0x7f800000u) sh = 13 - ilogbf(__uint_as_float(top));
-            const float f0 = ldexpf(1.f, sh / 2), f1 = ldexpf(1.f, sh - sh / 2);
-            const int mt = r >> 4, gg = r & 7, hi = (r >> 3) & 1;
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // the row's largest magnitude becomes 2^13 .. 2^14 (zeros, infinities and NaN: left)
+            const uint32_t tb = __float_as_uint(Half<DT>::to_f((uint16_t)top));
+            const int sh = tb != 0 && tb < 0x7f800000u ? 13 - ilogbf(__uint_as_float(tb)) : 0;
+            const float f0 = ldexpf(1.f, sh / 2), f1 = ldexpf(1.f, sh - sh / 2);  // two steps: 2^sh can leave fp32
 #pragma unroll
-            for (int e = 0; e < EPL; e += 2) {
-                const int d = lane * EPL + e;
-                const int ks = (d / 64) * 4 + (d % 16) / 4, cc = (d % 64) / 16, reg = ((d % 4) >> 1) * 2 + hi;
-                reinterpret_cast<uint32_t*>(s_q + (ks * MT + mt) * 32 + gg * 4 + cc)[reg] =
-                    f16x2(f[e] * f0 * f1, f[e + 1] * f0 * f1);
+            for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    f[i * 4 + w][0] = f16x2(e[i][4 * w] * f0 * f1, e[i][4 * w + 1] * f0 * f1);
+                    f[i * 4 + w][1] = f16x2(e[i][4 * w + 2] * f0 * f1, e[i][4 * w + 3] * f0 * f1);
+                }
+            return ldexpf(a.scale_log2, -sh);
+        };
+        if (kSharedQ) {
+            if (warp < NB) {
+                uint32_t f[KS][2];
+                const float v = load_q(warp, f);
+#pragma unroll
+                for (int k = 0; k < KS; ++k) s_q[(k * NB + warp) * 32 + lane] = make_uint2(f[k][0], f[k][1]);
+                if (c == 0) s_fac[8 * warp + g] = v;
             }
-            if (lane == 0) s_fac[r] = ldexpf(a.scale_log2, -sh);
+            __syncthreads();
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                fac[nb][0] = s_fac[8 * nb + 2 * c];
+                fac[nb][1] = s_fac[8 * nb + 2 * c + 1];
+            }
+        } else {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const float v = load_q(nb, qf[kSharedQ ? 0 : nb]);
+                fac[nb][0] = __shfl_sync(0xffffffffu, v, 8 * c);
+                fac[nb][1] = __shfl_sync(0xffffffffu, v, 8 * c + 4);
+            }
         }
-        __syncthreads();
 
-        float fac[MT][2], m[MT][2], l[MT][2], o[MT][NT][4];
-        int key_hi[MT][2], key_lo[MT][2];
+        // rows 2c, 2c + 1 of each 8: maximum, this lane's part of the sum, outputs
+        float m[NB][2], l[NB][2], o[NB][MD][4];
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int nb = 0; nb < NB; ++nb) {
+            m[nb][0] = m[nb][1] = -INFINITY;
+            l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = 16 * t + 8 * e + g;
-                fac[t][e] = s_fac[r];
-                m[t][e] = -INFINITY;
-                l[t][e] = 0.f;
-                const int pos = sq.past + (row0 + r) / a.G;
-                key_hi[t][e] = r < span.rows ? pos + 1 : 0;
-                key_lo[t][e] = a.window > 0 ? pos - a.window + 1 : 0;
-            }
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
+            for (int k = 0; k < MD; ++k) o[nb][k][0] = o[nb][k][1] = o[nb][k][2] = o[nb][k][3] = 0.f;
+        }
         // keys that every row of the block sees
         const int all_hi = sq.past + row0 / a.G + 1;
         const int all_lo = a.window > 0 ? sq.past + (row0 + span.rows - 1) / a.G - a.window + 1 : 0;
 
         int slot = 0;
         for (int it = 0; warp + kWarps * it < n_items; ++it) {
-            const float ks = sc0.x, vs = sc0.y;
-            sc0 = sc1;
-            sc1 = issue(it + 2, slot == 0 ? 2 : slot - 1);
-            cp_async_wait<2>();
+            const float ks = sc[0].x, vs = sc[0].y;
+#pragma unroll
+            for (int i = 0; i + 2 < kStages; ++i) sc[i] = sc[i + 1];
+            sc[kStages - 2] = issue(it + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);
+            cp_async_wait<kStages - 1>();
             __syncwarp();
-            const int item = warp + kWarps * it;
-            const int t0 = (span.lo + pa) * kPage + item * 32;
+            const int t0 = (span.lo + pa) * kPage + (warp + kWarps * it) * 32;
             const unsigned char* st = ring + slot * kStage;
             if (++slot == kStages) slot = 0;
             if (!(t0 < keys_hi && t0 + 32 > keys_lo)) continue;
 
-            // scores of 32 tokens: column n of tile j is token 8 (n / 2) + 2 j + n % 2
-            float s[MT][4][4];
+            // scores of 32 tokens: row g of group q (tile q / 2, its half q % 2) is token 8 (g / 2) + 2 q + g % 2
+            float s[NB][2][4];
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[t][j][0] = s[t][j][1] = s[t][j][2] = s[t][j][3] = 0.f;
+                for (int t = 0; t < 2; ++t) s[nb][t][0] = s[nb][t][1] = s[nb][t][2] = s[nb][t][3] = 0.f;
+            const unsigned char* krow = st + (8 * (g >> 1) + (g & 1)) * D;
 #pragma unroll
             for (int i = 0; i < D / 64; ++i) {
                 uint4 kw[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int row = 8 * (g >> 1) + 2 * j + (g & 1), ch = c + 4 * i;
-                    kw[j] = *reinterpret_cast<const uint4*>(st + row * D + (D == 128 ? ch ^ ((row & 1) << 2) : ch) * 16);
+                for (int q = 0; q < 4; ++q) {
+                    const int ch = c + 4 * i;
+                    kw[q] = *reinterpret_cast<const uint4*>(krow + q * 2 * D + (D == 128 ? ch ^ ((g & 1) << 2) : ch) * 16);
                 }
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    uint4 qa[MT];
+                    uint32_t lo[4], hi[4];
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) qa[t] = s_q[((i * 4 + w) * MT + t) * 32 + lane];
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t word = w == 0 ? kw[q].x : w == 1 ? kw[q].y : w == 2 ? kw[q].z : kw[q].w;
+                        lo[q] = codes_f16x2(word, 0x4140);
+                        hi[q] = codes_f16x2(word, 0x4342);
+                    }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t word = w == 0 ? kw[j].x : w == 1 ? kw[j].y : w == 2 ? kw[j].z : kw[j].w;
-                        const uint32_t b0 = codes_f16x2(word, 0x4140), b1 = codes_f16x2(word, 0x4342);
-#pragma unroll
-                        for (int t = 0; t < MT; ++t) mma_f16(s[t][j], qa[t], b0, b1);
+                    for (int nb = 0; nb < NB; ++nb) {
+                        uint2 qb;
+                        if (kSharedQ) qb = s_q[((i * 4 + w) * NB + nb) * 32 + lane];
+                        else qb = make_uint2(qf[kSharedQ ? 0 : nb][i * 4 + w][0], qf[kSharedQ ? 0 : nb][i * 4 + w][1]);
+                        mma_f16(s[nb][0], lo[0], lo[1], hi[0], hi[1], qb.x, qb.y);
+                        mma_f16(s[nb][1], lo[2], lo[3], hi[2], hi[3], qb.x, qb.y);
                     }
                 }
             }
             // weights: x = fac ks (q.c) + log2 vs; a page of zeros (scale 0) keeps its weight in the sum
             const float lv = vs == 0.f ? 0.f : __log2f(vs), iv = vs == 0.f ? 1.f : __fdividef(1.f, vs);
             const bool inside = t0 + 32 <= all_hi && t0 >= all_lo;
-            uint4 p[MT][2];
+            uint32_t p[NB][4];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                float mx[2] = {-INFINITY, -INFINITY};
-                const float al[2] = {fac[t][0] * ks, fac[t][1] * ks};
+            for (int nb = 0; nb < NB; ++nb) {
+                const float al[2] = {fac[nb][0] * ks, fac[nb][1] * ks};
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[t][j][e] = fmaf(s[t][j][e], al[e >> 1], lv);
+                    for (int e = 0; e < 4; ++e) s[nb][t][e] = fmaf(s[nb][t][e], al[e & 1], lv);
                 if (!inside) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = 8 * nb + 2 * c + e, pos = sq.past + (row0 + r) / a.G;
+                        const int khi = r < span.rows ? pos + 1 : 0, klo = a.window > 0 ? pos - a.window + 1 : 0;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int tok = t0 + 8 * c + 2 * j + (e & 1);
-                            if (tok >= key_hi[t][e >> 1] || tok < key_lo[t][e >> 1]) s[t][j][e] = -INFINITY;
+                        for (int q = 0; q < 4; ++q) {
+                            const int tok = t0 + 8 * (g >> 1) + 2 * q + (g & 1);
+                            if (tok >= khi || tok < klo) s[nb][q >> 1][(q & 1) * 2 + e] = -INFINITY;
                         }
+                    }
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[t][j][e]);
                 float corr[2], off[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-                    mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-                    const float nm = fmaxf(m[t][e], mx[e]);
-                    corr[e] = nm == m[t][e] ? 1.f : ex2(m[t][e] - nm);  // (also for -inf so far)
-                    m[t][e] = nm;
+                    float mx = fmaxf(fmaxf(s[nb][0][e], s[nb][0][2 + e]), fmaxf(s[nb][1][e], s[nb][1][2 + e]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float nm = fmaxf(m[nb][e], mx);
+                    corr[e] = nm == m[nb][e] ? 1.f : ex2(m[nb][e] - nm);  // (also for -inf so far)
+                    m[nb][e] = nm;
                     off[e] = 15.f - (nm == -INFINITY ? 0.f : nm);
                 }
-                float ps[2] = {0.f, 0.f};
+                float ps[2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[t][j][e] = ex2(s[t][j][e] + off[e >> 1]);
-                        ps[e >> 1] += s[t][j][e];
-                    }
-#pragma unroll
-                for (int e = 0; e < 2; ++e)  // a row that sees nothing of this page takes nothing of its scale either
-                    l[t][e] = l[t][e] * corr[e] + (ps[e] == 0.f ? 0.f : ps[e] * iv);
+                    for (int q = 0; q < 4; ++q) s[nb][q >> 1][(q & 1) * 2 + e] = ex2(s[nb][q >> 1][(q & 1) * 2 + e] + off[e]);
+                    ps[e] = (s[nb][0][e] + s[nb][0][2 + e]) + (s[nb][1][e] + s[nb][1][2 + e]);
+                    // a row that sees nothing of this page takes nothing of its scale either
+                    l[nb][e] = l[nb][e] * corr[e] + (ps[e] == 0.f ? 0.f : ps[e] * iv);
+                }
                 if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        o[t][n][0] *= corr[0];
-                        o[t][n][1] *= corr[0];
-                        o[t][n][2] *= corr[1];
-                        o[t][n][3] *= corr[1];
+                    for (int k = 0; k < MD; ++k) {
+                        o[nb][k][0] *= corr[0];
+                        o[nb][k][1] *= corr[1];
+                        o[nb][k][2] *= corr[0];
+                        o[nb][k][3] *= corr[1];
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    p[t][k].x = f16x2(s[t][2 * k][0], s[t][2 * k][1]);
-                    p[t][k].y = f16x2(s[t][2 * k][2], s[t][2 * k][3]);
-                    p[t][k].z = f16x2(s[t][2 * k + 1][0], s[t][2 * k + 1][1]);
-                    p[t][k].w = f16x2(s[t][2 * k + 1][2], s[t][2 * k + 1][3]);
-                }
+                for (int q = 0; q < 4; ++q)
+                    p[nb][q] = transpose8(f16x2(s[nb][q >> 1][(q & 1) * 2], s[nb][q >> 1][(q & 1) * 2 + 1]));
             }
+            // outputs: dimensions 16 k + g and + 8, tokens 8 c .. 8 c + 7 of the half page
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const uint2 vw = *reinterpret_cast<const uint2*>(st + kKBytes + (8 * n + g) * 32 + c * 8);
-                const uint32_t b0 = codes_f16x2(vw.x, 0x4140), b1 = codes_f16x2(vw.x, 0x4342);
-                const uint32_t b2 = codes_f16x2(vw.y, 0x4140), b3 = codes_f16x2(vw.y, 0x4342);
+            for (int k = 0; k < MD; ++k) {
+                const uint2 v0 = *reinterpret_cast<const uint2*>(st + kKBytes + (16 * k + g) * 32 + c * 8);
+                const uint2 v1 = *reinterpret_cast<const uint2*>(st + kKBytes + (16 * k + g + 8) * 32 + c * 8);
+                const uint32_t a0 = codes_f16x2(v0.x, 0x4140), a1 = codes_f16x2(v1.x, 0x4140);
+                const uint32_t a2 = codes_f16x2(v0.x, 0x4342), a3 = codes_f16x2(v1.x, 0x4342);
+                const uint32_t a4 = codes_f16x2(v0.y, 0x4140), a5 = codes_f16x2(v1.y, 0x4140);
+                const uint32_t a6 = codes_f16x2(v0.y, 0x4342), a7 = codes_f16x2(v1.y, 0x4342);
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    mma_f16(o[t][n], p[t][0], b0, b1);
-                    mma_f16(o[t][n], p[t][1], b2, b3);
+                for (int nb = 0; nb < NB; ++nb) {
+                    mma_f16(o[nb][k], a0, a1, a2, a3, p[nb][0], p[nb][1]);
+                    mma_f16(o[nb][k], a4, a5, a6, a7, p[nb][2], p[nb][3]);
                 }
             }
             __syncwarp();  // the stage is free for the copies issued next
@@ -392,38 +459,36 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
         cp_async_wait<0>();
 
         // ---- join the warps -----------------------------------------------------
-        __syncthreads();  // the rings become the joined results' buffer
+        // (a warp without items has -inf, 0 and zeros)
+        __syncthreads();  // the rings become the results' buffer
+        const int busy = min(kWarps, n_items);
+        if (warp < busy) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = 16 * t + 8 * e + g;
-                l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 1);
-                l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 2);
-                if (c == 0) {
-                    s_m[warp * RB + r] = m[t][e];
-                    s_l[warp * RB + r] = l[t][e];
+                for (int e = 0; e < 2; ++e) {
+                    const int r = 8 * nb + 2 * c + e;
+                    l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 4);
+                    l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 8);
+                    l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 16);
+                    if (g == 0) {
+                        s_m[warp * RB + r] = m[nb][e];
+                        s_l[warp * RB + r] = l[nb][e];
+                    }
+                    if (r < span.rows) {
+                        float* dst = s_o + (warp * RB + r) * kOPitch + g;
+#pragma unroll
+                        for (int k = 0; k < MD; ++k) {
+                            dst[16 * k] = o[nb][k][e];
+                            dst[16 * k + 8] = o[nb][k][2 + e];
+                        }
+                    }
                 }
-                if (r < span.rows) {
-                    float* dst = s_o + (warp * RB + r) * kOPitch + 2 * c;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(o[t][n][2 * e], o[t][n][2 * e + 1]);
-                }
-            }
+        }
         __syncthreads();
         const bool whole = pa == 0 && pb == np;
-        const long long hend = hb + np;
         // blocks that share this (segment, head)
-        int cf = blockIdx.x, cl = blockIdx.x;
-        if (!whole) {
-            cf = (int)(hb * nblk / U);
-            while (share(cf + 1) <= hb) ++cf;
-            while (share(cf) > hb) --cf;
-            cl = (int)((hend - 1) * nblk / U);
-            while (share(cl + 1) < hend) ++cl;
-            while (share(cl) >= hend) --cl;
-        }
+        const int cf = whole ? blockIdx.x : owner(hb), cl = whole ? blockIdx.x : owner(hb + np - 1);
         constexpr int kPart = kMaxRows * 128 + 2 * kMaxRows;
         float* part = a.parts + (long long)(2 * blockIdx.x + (u != u0)) * kPart;
         constexpr int Q4 = D / 4;
@@ -438,12 +503,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
         for (int i = tid; i < span.rows * Q4; i += kThreads) {
             const int r = i / Q4, q4 = i % Q4;
             float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w * RB + r]);
+            for (int w = 0; w < busy; ++w) top = fmaxf(top, s_m[w * RB + r]);
             float sl = 0.f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
+#pragma unroll 4
+            for (int w = 0; w < busy; ++w) {
                 const float mw = s_m[w * RB + r];
                 const float f = mw == -INFINITY ? 0.f : ex2(mw - top);
                 const float4 v = *reinterpret_cast<const float4*>(s_o + (w * RB + r) * kOPitch + 4 * q4);
@@ -475,25 +539,47 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
             }
             __syncthreads();
             if (s_last) {
+                // a block's piece is its first one (slot 0) unless its share begins before this head
+                const float* p0 = a.parts + (long long)(2 * cf + (share(cf) < hb)) * kPart;
+                const float* p1 = a.parts + (long long)(2 * cf + 2) * kPart;  // of block cf + 1, then every second slot
                 for (int i = tid; i < span.rows * Q4; i += kThreads) {
                     const int r = i / Q4, q4 = i % Q4;
-                    // the last block's piece is its first unless its share begins before this head
-                    auto at = [&](int k) { return a.parts + (long long)(2 * k + (k == cf && share(cf) < hb)) * kPart; };
                     float top = -INFINITY, sl = 0.f;
                     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int k = cf; k <= cl; ++k) top = fmaxf(top, __ldcg(at(k) + kMaxRows * 128 + r));
-#pragma unroll 4
-                    for (int k = cf; k <= cl; ++k) {
-                        const float* pk = at(k);
-                        const float mk = __ldcg(pk + kMaxRows * 128 + r);
-                        const float f = mk == -INFINITY ? 0.f : ex2(mk - top);
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(pk + r * D + 4 * q4));
-                        sl += __ldcg(pk + kMaxRows * 128 + kMaxRows + r) * f;
-                        acc.x += v.x * f;
-                        acc.y += v.y * f;
-                        acc.z += v.z * f;
-                        acc.w += v.w * f;
+                    for (int k0 = 0; k0 <= cl - cf; k0 += 8) {  // eight pieces' loads at a time
+                        float mk[8], lk[8];
+                        float4 v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float* pk = k0 + k == 0 ? p0 : p1 + (long long)(2 * (k0 + k - 1)) * kPart;
+                            mk[k] = -INFINITY;
+                            lk[k] = 0.f;
+                            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (k0 + k <= cl - cf) {
+                                mk[k] = __ldcg(pk + kMaxRows * 128 + r);
+                                lk[k] = __ldcg(pk + kMaxRows * 128 + kMaxRows + r);
+                                v[k] = __ldcg(reinterpret_cast<const float4*>(pk + r * D + 4 * q4));
+                            }
+                        }
+                        float nt = top;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) nt = fmaxf(nt, mk[k]);
+                        const float back = nt == top ? 1.f : ex2(top - nt);
+                        sl *= back;
+                        acc.x *= back;
+                        acc.y *= back;
+                        acc.z *= back;
+                        acc.w *= back;
+                        top = nt;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float f = mk[k] == -INFINITY ? 0.f : ex2(mk[k] - top);
+                            sl += lk[k] * f;
+                            acc.x += v[k].x * f;
+                            acc.y += v[k].y * f;
+                            acc.z += v[k].z * f;
+                            acc.w += v[k].w * f;
+                        }
                     }
                     finish(r, q4, acc, sl);
                 }
@@ -505,15 +591,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
     pdl_launch_dependents();
 }
 
-template <int DT, int D, int MT>
+template <int DT, int D, int NB>
 int launch(const AttnArgs& a, int grid, momij_stream_t st) {
-    constexpr int RB = 16 * MT;
-    constexpr size_t ring = (size_t)kWarps * kStages * (2 * 32 * D), join = (size_t)kWarps * RB * (D + 4) * 4;
-    const size_t smem = (ring > join ? ring : join) + (D / 16) * MT * 512 + RB * 4 + 2 * kWarps * RB * 4 +
+    constexpr int RB = 8 * NB, W = Shape<NB>::kWarps;
+    constexpr size_t ring = (size_t)W * Shape<NB>::kStages * 64 * D, join = (size_t)W * RB * (D + 4) * 4;
+    const size_t smem = (ring > join ? ring : join) + (NB == 4 ? (D / 16) * NB * 256 : 0) + RB * 4 + 2 * W * RB * 4 +
                         ((size_t)a.nb * a.nrb + 1) * 4;
     static int granted[64];
-    if (!host_allow_smem(attn_kernel<DT, D, MT>, smem, granted)) return MOMIJ_ERR_CUDA;
-    return host_launch(attn_kernel<DT, D, MT>, dim3(grid), dim3(kThreads), smem, st, a);
+    if (!host_allow_smem(attn_kernel<DT, D, NB>, smem, granted)) return MOMIJ_ERR_CUDA;
+    return host_launch(attn_kernel<DT, D, NB>, dim3(grid), dim3(W * 32), smem, st, a);
+}
+template <int DT, int D>
+int launch_rows(const AttnArgs& a, int rows, int grid, momij_stream_t st) {
+    if (rows == 8) return launch<DT, D, 1>(a, grid, st);
+    if (rows == 16) return launch<DT, D, 2>(a, grid, st);
+    return launch<DT, D, 4>(a, grid, st);
 }
 
 size_t part_bytes(int sms) { return (size_t)2 * sms * (kMaxRows * 128 + 2 * kMaxRows) * 4; }
@@ -580,25 +672,25 @@ extern "C" int momij_attention(const void* q, long long ldq, void* out, long lon
     a.table_cols = table_cols;
     a.window = window;
     a.longest = cu_q ? (max_q > 0 ? std::min(max_q, T) : T) : T / B;
+    a.qvec = host_aligned(q, 16) && ldq % 8 == 0;
     a.spin = host_spin_limit();
     a.scale_log2 = scale * 1.4426950408889634f;
     const long long rows = (long long)a.longest * a.G;
-    const int mt = rows <= 16 ? 1 : 2;
-    const long long nrb = (rows + 16 * mt - 1) / (16 * mt);
-    if (nrb > kMaxSeg) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
+    const int rb = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+    const long long nrb = (rows + rb - 1) / rb;
+    // sequences per launch: their row blocks and units (row block, head, page) stay countable
+    const long long units = nrb * Hkv * std::max(table_cols, 1);
+    if (nrb > kMaxSeg || units > (1LL << 30)) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     a.nrb = (int)nrb;
-    const int per = std::max(1, kMaxSeg / a.nrb);  // sequences per launch
+    const int per = (int)std::min<long long>(kMaxSeg / nrb, (1LL << 30) / units);
     for (int b = 0; b < B; b += per) {
         a.b0 = b;
         a.nb = std::min(per, B - b);
         int rc;
-        if (dtype == MOMIJ_DTYPE_BF16) {
-            if (D == 64) rc = mt == 1 ? launch<MOMIJ_DTYPE_BF16, 64, 1>(a, sms, stream) : launch<MOMIJ_DTYPE_BF16, 64, 2>(a, sms, stream);
-            else rc = mt == 1 ? launch<MOMIJ_DTYPE_BF16, 128, 1>(a, sms, stream) : launch<MOMIJ_DTYPE_BF16, 128, 2>(a, sms, stream);
-        } else {
-            if (D == 64) rc = mt == 1 ? launch<MOMIJ_DTYPE_F16, 64, 1>(a, sms, stream) : launch<MOMIJ_DTYPE_F16, 64, 2>(a, sms, stream);
-            else rc = mt == 1 ? launch<MOMIJ_DTYPE_F16, 128, 1>(a, sms, stream) : launch<MOMIJ_DTYPE_F16, 128, 2>(a, sms, stream);
-        }
+        if (dtype == MOMIJ_DTYPE_BF16)
+            rc = D == 64 ? launch_rows<MOMIJ_DTYPE_BF16, 64>(a, rb, sms, stream) : launch_rows<MOMIJ_DTYPE_BF16, 128>(a, rb, sms, stream);
+        else
+            rc = D == 64 ? launch_rows<MOMIJ_DTYPE_F16, 64>(a, rb, sms, stream) : launch_rows<MOMIJ_DTYPE_F16, 128>(a, rb, sms, stream);
         if (rc) return rc;
     }
     return MOMIJ_OK;

@@ -18,6 +18,7 @@ struct AttnArgs {
     long long ldq, ldo;
     int T, B, Hq, Hkv, G, n_pages, table_cols, window, longest;
     int b0, nb, nrb;     // sequences of this launch, row blocks per sequence
+    int qvec;            // q rows start on 16-byte boundaries
     int spin;
     float scale_log2;    // softmax scale * log2(e)
 };
