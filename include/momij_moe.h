@@ -268,17 +268,18 @@ int momij_moe_block(void* h, const void* norm_w, float eps, const void* w_gate, 
  * sequence (0: unknown, up to T).  lens, cu_q and block_table are read on the
  * device; a page, length or row outside its range is skipped and reported as
  * MOMIJ_ERR_PAGE by momij_moe_synchronize(stream, workspace).  D is 64 or 128,
- * Hq a multiple of Hkv.  Codes and the rotation table start on 16-byte
- * boundaries, 16-bit rows on 8-byte boundaries (attention's q: any).
+ * Hq a multiple of Hkv.  Codes, the rotation table, norm weights and rows of qkv, q_out,
+ * k_out and v_out start on 16-byte boundaries, attention's out rows on 8-byte
+ * boundaries (its q: any).
  */
 #define MOMIJ_KV_PAGE 64
 
 /* Head norms, rotation and append in one launch.  Row t of qkv (ld elements
- * apart, ld % 4 == 0) holds Hq query, Hkv key and Hkv value heads of D:
+ * apart, ld % 8 == 0) holds Hq query, Hkv key and Hkv value heads of D:
  *   y = x * rsqrt(mean(x^2) + eps) * weight          (queries, keys; weight [D], NULL: no norm)
  *   the first rot elements of y turn by the angles of the token's position
  *   (rope fp32 [rope_rows, rot]: rot/2 cosines, then rot/2 sines; pairs
- *   (i, i + rot/2), or (2i, 2i + 1) if interleaved; rot % 8 == 0, 0: none)
+ *   (i, i + rot/2), or (2i, 2i + 1) if interleaved; rot % 16 == 0, 0: none)
  * q_out [T, Hq, D] gets the queries; keys and values become codes at positions
  * lens[b] - n_b .. lens[b] - 1.  A page's scale is amax / 127 over its tokens so
  * far; when new tokens raise it, the page's earlier tokens are recoded (rounded

@@ -19,7 +19,8 @@
 // stay in registers between the maximum and the coding.  K rows are written
 // as they lie; V is turned through shared memory, so that a page's 64 tokens
 // of one dimension leave as 16-byte stores.  Query heads are spread over the
-// remaining blocks, half a warp or a warp a row.
+// remaining blocks, several heads of a token to a warp, which share the token's
+// weights times cosines and sines.
 //
 // What bounds it: bytes (the rows read once, queries and codes written once)
 // for a prompt's chunk, the launch for single tokens.
@@ -35,7 +36,7 @@ constexpr int kThreads = 256, kWarps = 8;
 // Pages whose scale would be smaller (values below 7e-18) read as zeros, so that
 // the attention's sums of weights divided by scales stay within fp32.
 constexpr float kMinScale = 0x1p-64f;
-constexpr int kQRows = 4;               // query rows per warp lane group
+constexpr int kQRows = 4;  // heads per lane group of a query warp
 
 struct AppendArgs {
     const uint16_t* qkv;
@@ -48,7 +49,7 @@ struct AppendArgs {
     int32_t* ws;
     const int32_t* stop;
     long long ld;             // elements between token rows of qkv
-    int T, B, Hq, Hkv, n_pages, table_cols, rot, rope_rows, interleaved, touched, kv_blocks, longest;
+    int T, B, Hq, Hkv, n_pages, table_cols, rot, rope_rows, interleaved, touched, kv_blocks, longest, q_chunks;
     float eps;
 };
 
@@ -72,66 +73,126 @@ __device__ __forceinline__ bool usable(const AppendArgs& a, const Seq& s) {
     return s.n >= 0 && s.n <= a.longest && s.past >= 0 && s.t0 >= 0 && s.n <= a.T - s.t0 && (!a.rope || s.past + s.n <= a.rope_rows);
 }
 
+// Two 16-bit values of a word as floats, and two floats rounded into one.
 template <int DT>
-__device__ __forceinline__ float4 load4h(const uint16_t* p) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    return make_float4(Half<DT>::to_f((uint16_t)(v.x & 0xffffu)), Half<DT>::to_f((uint16_t)(v.x >> 16)),
-                       Half<DT>::to_f((uint16_t)(v.y & 0xffffu)), Half<DT>::to_f((uint16_t)(v.y >> 16)));
+__device__ __forceinline__ float2 unpack(uint32_t w) {
+    return make_float2(Half<DT>::to_f((uint16_t)(w & 0xffffu)), Half<DT>::to_f((uint16_t)(w >> 16)));
 }
+template <int DT>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    if (DT == MOMIJ_DTYPE_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// Norm and rotation of one head row held four elements a lane (L lanes a row).
+// A head row lies in L = D / 8 lanes, eight elements each.  Norm and rotation
+// are one linear map of the raw row, scaled by its inverse root mean square:
+//   y_j = inv * (x_j * A_j + x'_j * B_j),  A = w cos,  B = +-w' sin
+// with x' (weight w') the element that x_j turns with.  A and B depend on the
+// position alone, so the heads of a token share them.
+struct Turn {
+    float A[8], B[8];
+};
 template <int DT, int L>
-__device__ __forceinline__ float4 norm_rotate(float4 x, const uint16_t* w, const float* table, int rot, int interleaved, int l,
-                                              float eps) {
+__device__ __forceinline__ Turn turn_of(const uint16_t* w, const float* table, int rot, int interleaved, int l) {
+    Turn t;
+    const int half = rot >> 1, step = rot >> 4;  // a half's lanes
+    const bool in = 8 * l < rot, first = l < step;
+    const int other = interleaved || !in ? l : first ? l + step : l - step;
+    uint4 g = make_uint4(0u, 0u, 0u, 0u), p = g;
     if (w) {
-        float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = rsqrtf(ss * (1.f / (4 * L)) + eps);
-        const float4 g = load4h<DT>(w + 4 * l);
-        x.x = x.x * inv * g.x;
-        x.y = x.y * inv * g.y;
-        x.z = x.z * inv * g.z;
-        x.w = x.w * inv * g.w;
+        g = __ldg(reinterpret_cast<const uint4*>(w) + l);
+        p = __ldg(reinterpret_cast<const uint4*>(w) + other);
     }
-    if (rot) {
-        const int half = rot >> 1;
-        if (interleaved) {
-            if (4 * l < rot) {
-                const float2 cs = __ldg(reinterpret_cast<const float2*>(table + 2 * l));
-                const float2 sn = __ldg(reinterpret_cast<const float2*>(table + half + 2 * l));
-                x = make_float4(x.x * cs.x - x.y * sn.x, x.y * cs.x + x.x * sn.x, x.z * cs.y - x.w * sn.y,
-                                x.w * cs.y + x.z * sn.y);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = w ? unpack<DT>(word(g, i)) : make_float2(1.f, 1.f);
+        const float2 b = w ? unpack<DT>(word(p, i)) : make_float2(1.f, 1.f);
+        t.A[2 * i] = a.x;
+        t.A[2 * i + 1] = a.y;
+        t.B[2 * i] = interleaved ? b.y : b.x;
+        t.B[2 * i + 1] = interleaved ? b.x : b.y;
+    }
+    if (in) {
+        if (interleaved) {  // pairs (2i, 2i + 1): four angles a lane
+            const float4 cs = __ldg(reinterpret_cast<const float4*>(table + 4 * l));
+            const float4 sn = __ldg(reinterpret_cast<const float4*>(table + half + 4 * l));
+            const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                t.A[j] *= cv[j >> 1];
+                t.B[j] *= j & 1 ? sv[j >> 1] : -sv[j >> 1];
             }
         } else {
-            // lanes of the first half (elements 4l < half) meet those rot/8 further on
-            const int step = rot >> 3;
-            const bool first = l < step, in = l < 2 * step;
-            const int base = (threadIdx.x & 31) & ~(L - 1);
-            const int src = base + (first ? l + step : in ? l - step : l);
-            const float4 o = make_float4(__shfl_sync(0xffffffffu, x.x, src), __shfl_sync(0xffffffffu, x.y, src),
-                                         __shfl_sync(0xffffffffu, x.z, src), __shfl_sync(0xffffffffu, x.w, src));
-            if (in) {
-                const int i = first ? 4 * l : 4 * (l - step);
-                const float4 cs = __ldg(reinterpret_cast<const float4*>(table + i));
-                float4 sn = __ldg(reinterpret_cast<const float4*>(table + half + i));
-                if (first) sn = make_float4(-sn.x, -sn.y, -sn.z, -sn.w);
-                x = make_float4(x.x * cs.x + o.x * sn.x, x.y * cs.y + o.y * sn.y, x.z * cs.z + o.z * sn.z,
-                                x.w * cs.w + o.w * sn.w);
+            const int i = 8 * (first ? l : l - step);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float4 cs = __ldg(reinterpret_cast<const float4*>(table + i) + k);
+                const float4 sn = __ldg(reinterpret_cast<const float4*>(table + half + i) + k);
+                const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    t.A[4 * k + j] *= cv[j];
+                    t.B[4 * k + j] *= first ? -sv[j] : sv[j];
+                }
             }
         }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t.B[j] = 0.f;
     }
-    return x;
+    return t;
+}
+// The turned row; norm: with the inverse root mean square, else 1.
+template <int DT, int L>
+__device__ __forceinline__ void norm_rotate(const uint4& raw, const Turn& t, bool norm, float eps, int rot, int interleaved, int l,
+                                            float (&y)[8]) {
+    float inv = 1.f;
+    if (norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack<DT>(word(raw, i));
+            ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
+        }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        inv = rsqrtf(ss * (1.f / (8 * L)) + eps);
+    }
+    const int step = rot >> 4;
+    const int src = (threadIdx.x & 31 & ~(L - 1)) + (l < step ? l + step : l < 2 * step ? l - step : l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = word(raw, i);
+        uint32_t o = w;
+        if (rot) o = interleaved ? __byte_perm(w, 0, 0x1032) : __shfl_sync(0xffffffffu, w, src);
+        const float2 f = unpack<DT>(w), q = unpack<DT>(o);
+        y[2 * i] = f.x * t.A[2 * i];
+        y[2 * i + 1] = f.y * t.A[2 * i + 1];
+        if (8 * l < rot) {
+            y[2 * i] = fmaf(q.x, t.B[2 * i], y[2 * i]);
+            y[2 * i + 1] = fmaf(q.y, t.B[2 * i + 1], y[2 * i + 1]);
+        }
+        y[2 * i] *= inv;
+        y[2 * i + 1] *= inv;
+    }
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
-// A code 128 + rint(x / scale), held to 1 .. 255.  Of a page with a NaN scale
-// the codes do not matter; they stay in range.
-__device__ __forceinline__ uint32_t code_of(float x, float inv) {
-    return (uint32_t)(128 + __float2int_rn(fminf(fmaxf(x * inv, -127.f), 127.f)));
+// Codes 128 + rint(x / scale) of four values: the addition of 1.5 * 2^23 + 128
+// rounds to a whole number (ties to even) and leaves it in the low byte; |x| /
+// scale is at most 127 and a rounding error.  (Of a page with a NaN scale the
+// codes do not matter.)
+__device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(fmaf(x[i], inv, 12583040.f));
+    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 __device__ __forceinline__ uint32_t recode(uint32_t byte, float ratio) {
-    return (uint32_t)(128 + __float2int_rn(fminf(fmaxf(((float)(int)byte - 128.f) * ratio, -127.f), 127.f)));
+    return __float_as_uint(fmaf((float)(int)byte - 128.f, ratio, 12583040.f)) & 255u;
 }
 __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
     return recode(w & 255u, ratio) | (recode((w >> 8) & 255u, ratio) << 8) | (recode((w >> 16) & 255u, ratio) << 16) |
@@ -140,13 +201,12 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
 
 template <int DT, int D>
 __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
-    constexpr int L = D / 4, RPW = 32 / L, ROWS = kWarps * RPW;  // lanes a row, rows a warp, rows a sweep
+    constexpr int L = D / 8, RPW = 32 / L, ROWS = kWarps * RPW;  // lanes a row, rows a warp, rows a sweep
     constexpr int SWEEPS = kPage / ROWS;
     constexpr int VP = kPage + 4;  // pitch of the turned V tile
     __shared__ __align__(16) uint8_t s_v[D * VP];
     __shared__ uint32_t s_top;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = lane % L;
-    const int row_in = warp * RPW + lane / L;  // this lane group's row within a sweep
     if (tid == 0) s_top = 0;
     pdl_wait();
     const int stopped = __syncthreads_or(tid == 0 && a.stop && __ldcg(a.stop) != 0);
@@ -154,48 +214,45 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
     if (stopped) return;
 
     if ((int)blockIdx.x >= a.kv_blocks) {
-        // ---- queries: rows (token, head), kQRows per lane group --------------
-        const long long rows = (long long)a.T * a.Hq;
-        const long long r0 = ((long long)(blockIdx.x - a.kv_blocks) * kQRows) * ROWS + row_in;
-        float4 x[kQRows];
+        // ---- queries: a warp takes RPW * kQRows heads of one token ---------------
+        const int w = (blockIdx.x - a.kv_blocks) * kWarps + warp, t = w / a.q_chunks;
+        if (t >= a.T) return;
+        const int h0 = (w - t * a.q_chunks) * (RPW * kQRows) + lane / L;
+        const uint16_t* src = a.qkv + t * a.ld + 8 * l;
+        uint4 raw[kQRows];
 #pragma unroll
         for (int i = 0; i < kQRows; ++i) {
-            const long long r = r0 + (long long)i * ROWS;
-            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < rows) x[i] = load4h<DT>(a.qkv + (r / a.Hq) * a.ld + (r % a.Hq) * D + 4 * l);
+            const int h = h0 + i * RPW;
+            raw[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (h < a.Hq) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + h * D));
         }
+        const float* table = a.rope;
+        if (a.rot) {
+            int b;
+            if (a.cu) {  // the sequence whose rows hold t
+                int lo = 0, hi = a.B - 1;
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (__ldg(a.cu + mid) <= t) lo = mid;
+                    else hi = mid - 1;
+                }
+                b = lo;
+            } else {
+                b = t / a.longest;
+            }
+            const Seq s = sequence(a, b);
+            if (!usable(a, s) || t < s.t0 || t >= s.t0 + s.n) return;  // (reported with the keys)
+            table += (long long)(s.past + t - s.t0) * a.rot;
+        }
+        const Turn turn = turn_of<DT, L>(a.qw, table, a.rot, a.interleaved, l);
 #pragma unroll
         for (int i = 0; i < kQRows; ++i) {
-            const long long r = r0 + (long long)i * ROWS;
-            const int t = (int)min(r / a.Hq, (long long)a.T - 1);
-            const float* table = a.rope;
-            bool fine = r < rows;
-            if (a.rot) {
-                int b;
-                if (a.cu) {  // the sequence whose rows hold t
-                    int lo = 0, hi = a.B - 1;
-                    while (lo < hi) {
-                        const int mid = (lo + hi + 1) >> 1;
-                        if (__ldg(a.cu + mid) <= t) lo = mid;
-                        else hi = mid - 1;
-                    }
-                    b = lo;
-                } else {
-                    b = t / (a.T / a.B);
-                }
-                const Seq s = sequence(a, b);
-                const int pos = s.past + t - s.t0;
-                const bool at = usable(a, s) && t >= s.t0 && t < s.t0 + s.n;
-                fine = fine && at;
-                table += (long long)(at ? pos : 0) * a.rot;
-            }
-            const float4 y = norm_rotate<DT, L>(x[i], a.qw, table, a.rot, a.interleaved, l, a.eps);
-            if (fine) {
-                uint2 o;
-                o.x = Half<DT>::from_f(y.x) | ((uint32_t)Half<DT>::from_f(y.y) << 16);
-                o.y = Half<DT>::from_f(y.z) | ((uint32_t)Half<DT>::from_f(y.w) << 16);
-                *reinterpret_cast<uint2*>(a.q + r * D + 4 * l) = o;
-            }
+            const int h = h0 + i * RPW;
+            float y[8];
+            norm_rotate<DT, L>(raw[i], turn, a.qw != nullptr, a.eps, a.rot, a.interleaved, l, y);
+            if (h < a.Hq)
+                *reinterpret_cast<uint4*>(a.q + ((long long)t * a.Hq + h) * D + 8 * l) =
+                    make_uint4(pack<DT>(y[0], y[1]), pack<DT>(y[2], y[3]), pack<DT>(y[4], y[5]), pack<DT>(y[6], y[7]));
         }
         pdl_launch_dependents();
         return;
@@ -221,32 +278,47 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
         if (tid == 0) cache_error(a.ws, MOMIJ_ERR_PAGE);
         return;
     }
-    const int r0 = lo - blk * kPage, r1 = hi - blk * kPage;  // rows of the page
+    const int r0 = lo - blk * kPage, nr = hi - lo;  // first row of the page, rows
     const long long ph = (long long)page * a.Hkv + h;
     float* scale_at = (is_v ? a.vs : a.ks) + ph;
-    const uint16_t* src = a.qkv + (long long)(s.t0 + lo - s.past) * a.ld + (long long)(a.Hq + h + (is_v ? a.Hkv : 0)) * D + 4 * l;
+    const int row_in = warp * RPW + lane / L;  // this lane's row within a sweep
+    const uint16_t* src = a.qkv + (long long)(s.t0 + lo - s.past) * a.ld + (long long)(a.Hq + h + (is_v ? a.Hkv : 0)) * D + 8 * l;
 
-    float4 x[SWEEPS];
-    uint32_t top = 0;
+    const float had = r0 > 0 ? __ldcg(scale_at) : 0.f;
+    uint4 raw[SWEEPS];
 #pragma unroll
     for (int i = 0; i < SWEEPS; ++i) {
         const int r = i * ROWS + row_in;
-        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < r1 - r0) x[i] = load4h<DT>(src + r * a.ld);
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < nr) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + r * a.ld));
     }
+    float x[SWEEPS][8];
+    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < SWEEPS; ++i) {
-        if (i * ROWS >= r1 - r0) break;
-        const int r = min(i * ROWS + row_in, r1 - r0 - 1);
-        if (!is_v) x[i] = norm_rotate<DT, L>(x[i], a.kw, a.rope + (long long)(lo + r) * a.rot, a.rot, a.interleaved, l, a.eps);
-        if (i * ROWS + row_in < r1 - r0)
-            top = max(top, max(max(abs_bits(x[i].x), abs_bits(x[i].y)), max(abs_bits(x[i].z), abs_bits(x[i].w))));
+        if (i * ROWS < nr) {
+            const int r = min(i * ROWS + row_in, nr - 1);
+            if (is_v) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 f = unpack<DT>(word(raw[i], k));
+                    x[i][2 * k] = f.x;
+                    x[i][2 * k + 1] = f.y;
+                }
+            } else {
+                const Turn turn = turn_of<DT, L>(a.kw, a.rope + (long long)(lo + r) * a.rot, a.rot, a.interleaved, l);
+                norm_rotate<DT, L>(raw[i], turn, a.kw != nullptr, a.eps, a.rot, a.interleaved, l, x[i]);
+            }
+            if (i * ROWS + row_in < nr) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = max(top, abs_bits(x[i][k]));
+            }
+        }
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0 && top) atomicMax(&s_top, top);
-    __syncthreads();
+    __syncthreads();  // (every thread has read the old scale, too)
     // The scale; infinities and NaN make it NaN, and the page reads as NaN.
-    const float had = r0 > 0 ? __ldcg(scale_at) : 0.f;
     float scale = __uint_as_float(s_top) * (1.f / 127.f);
     if (scale < kMinScale) scale = 0.f;
     if (s_top >= 0x7f800000u || !(had <= 3.0e38f)) scale = __int_as_float(0x7fffffff);
@@ -254,7 +326,6 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
     const float inv = scale > 0.f ? 1.f / scale : 0.f;
     const bool grew = r0 > 0 && scale > had;  // (false for a NaN scale: its codes do not matter)
     const float ratio = had * inv;
-    __syncthreads();  // every thread has read the old scale
     if (tid == 0) *scale_at = scale;
 
     if (!is_v) {
@@ -262,9 +333,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
 #pragma unroll
         for (int i = 0; i < SWEEPS; ++i) {
             const int r = i * ROWS + row_in;
-            if (r < r1 - r0)
-                *reinterpret_cast<uint32_t*>(dst + (r0 + r) * D + 4 * l) =
-                    code_of(x[i].x, inv) | (code_of(x[i].y, inv) << 8) | (code_of(x[i].z, inv) << 16) | (code_of(x[i].w, inv) << 24);
+            if (r < nr) *reinterpret_cast<uint2*>(dst + (r0 + r) * D + 8 * l) = make_uint2(codes4(x[i], inv), codes4(x[i] + 4, inv));
         }
         if (grew)
             for (int i = tid; i < r0 * D / 4; i += kThreads) {
@@ -276,16 +345,18 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
 #pragma unroll
         for (int i = 0; i < SWEEPS; ++i) {
             const int r = i * ROWS + row_in;
-            if (r < r1 - r0) {
-                uint8_t* t = s_v + 4 * l * VP + r0 + r;
-                t[0] = (uint8_t)code_of(x[i].x, inv);
-                t[VP] = (uint8_t)code_of(x[i].y, inv);
-                t[2 * VP] = (uint8_t)code_of(x[i].z, inv);
-                t[3 * VP] = (uint8_t)code_of(x[i].w, inv);
+            if (r < nr) {
+                uint8_t* t = s_v + 8 * l * VP + r0 + r;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t c = codes4(x[i] + 4 * k, inv);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) t[(4 * k + e) * VP] = (uint8_t)(c >> (8 * e));
+                }
             }
         }
         __syncthreads();
-        const int w0 = grew ? 0 : r0;  // rows [w0, r1) change
+        const int r1 = r0 + nr, w0 = grew ? 0 : r0;  // rows [w0, r1) change
         for (int i = tid; i < D * (kPage / 16); i += kThreads) {
             const int d = i >> 2, c0 = (i & 3) * 16, c1 = c0 + 16;
             if (c1 <= w0 || c0 >= r1) continue;
@@ -331,14 +402,14 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
     const int h = u % a.Hkv;
     u /= a.Hkv;
     const int j = u % a.parts, b = u / a.parts;
-    const long long f = a.first ? __ldg(a.first + b) : 0;
+    const long long from = a.first ? __ldg(a.first + b) : 0;
     const int len = __ldg(a.lens + b);
-    if (f < 0) {
+    if (from < 0) {
         if (tid == 0) cache_error(a.ws, MOMIJ_ERR_PAGE);
         return;
     }
-    const long long blk = f / kPage + j, p0 = blk * kPage;
-    const long long t0 = p0 > f ? p0 : f, t1 = p0 + kPage < f + a.count ? p0 + kPage : f + a.count;  // tokens asked for here
+    const long long blk = from / kPage + j, p0 = blk * kPage;
+    const long long t0 = p0 > from ? p0 : from, t1 = p0 + kPage < from + a.count ? p0 + kPage : from + a.count;  // tokens asked for here
     if (t0 >= t1) return;
     int page = -1;
     if (t0 < len) {
@@ -364,27 +435,28 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
         __syncthreads();
     }
     uint16_t* out = (is_v ? a.vo : a.ko) + ((long long)b * a.count * a.Hkv + h) * D;
-    constexpr int L = D / 4;
+    constexpr int L = D / 8;
+#pragma unroll
     for (int i = tid; i < kPage * L; i += kThreads) {
         const int r = i / L, l = i % L;
         const long long t = p0 + r;
         if (t < t0 || t >= t1) continue;
-        uint2 o = make_uint2(0u, 0u);
+        uint4 o = make_uint4(0u, 0u, 0u, 0u);
         if (t < len) {
-            uint32_t c;
+            uint2 c;
             if (is_v) {
-                const uint8_t* q = s_v + 4 * l * VP + r;
-                c = q[0] | ((uint32_t)q[VP] << 8) | ((uint32_t)q[2 * VP] << 16) | ((uint32_t)q[3 * VP] << 24);
+                const uint8_t* q = s_v + 8 * l * VP + r;
+                c.x = q[0] | ((uint32_t)q[VP] << 8) | ((uint32_t)q[2 * VP] << 16) | ((uint32_t)q[3 * VP] << 24);
+                c.y = q[4 * VP] | ((uint32_t)q[5 * VP] << 8) | ((uint32_t)q[6 * VP] << 16) | ((uint32_t)q[7 * VP] << 24);
             } else {
-                c = __ldg(reinterpret_cast<const uint32_t*>(src + r * D + 4 * l));
+                c = __ldg(reinterpret_cast<const uint2*>(src + r * D + 8 * l));
             }
-            float f4[4];
+            float f[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f4[e] = ((float)(int)((c >> (8 * e)) & 255u) - 128.f) * scale;
-            o.x = Half<DT>::from_f(f4[0]) | ((uint32_t)Half<DT>::from_f(f4[1]) << 16);
-            o.y = Half<DT>::from_f(f4[2]) | ((uint32_t)Half<DT>::from_f(f4[3]) << 16);
+            for (int e = 0; e < 8; ++e) f[e] = ((float)(int)(((e < 4 ? c.x : c.y) >> (8 * (e & 3))) & 255u) - 128.f) * scale;
+            o = make_uint4(pack<DT>(f[0], f[1]), pack<DT>(f[2], f[3]), pack<DT>(f[4], f[5]), pack<DT>(f[6], f[7]));
         }
-        *reinterpret_cast<uint2*>(out + (t - f) * ((long long)a.Hkv * D) + 4 * l) = o;
+        *reinterpret_cast<uint4*>(out + (t - from) * ((long long)a.Hkv * D) + 8 * l) = o;
     }
     pdl_launch_dependents();
 }
@@ -402,14 +474,14 @@ extern "C" int momij_qk_norm_rope_append(const void* qkv, long long ld, void* q_
     if (int rc = host_check_device()) return rc;
     if (T < 0 || B < 0 || n_pages < 0 || table_cols < 0 || rope_rows < 0 || max_q < 0) return MOMIJ_ERR_INVALID_ARGUMENT;
     if (dtype != MOMIJ_DTYPE_BF16 && dtype != MOMIJ_DTYPE_F16) return MOMIJ_ERR_INVALID_ARGUMENT;
-    if (Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || (D != 64 && D != 128) || rot < 0 || rot > D || rot % 8 != 0)
+    if (Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || (D != 64 && D != 128) || rot < 0 || rot > D || rot % 16 != 0)
         return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     if (T == 0 || B == 0) return MOMIJ_OK;
     if (!cu_q && T % B != 0) return MOMIJ_ERR_INVALID_ARGUMENT;
     if (!qkv || !q_out || !k_codes || !v_codes || !k_scales || !v_scales || !block_table || !lens || (rot && !rope))
         return MOMIJ_ERR_INVALID_ARGUMENT;
-    if (ld < (long long)(Hq + 2 * Hkv) * D || ld % 4 != 0 || !host_aligned(qkv, 8) || !host_aligned(q_out, 8) || !host_aligned(rope, 16) ||
-        !host_aligned(k_codes, 16) || !host_aligned(v_codes, 16) || !host_aligned(q_weight, 8) || !host_aligned(k_weight, 8))
+    if (ld < (long long)(Hq + 2 * Hkv) * D || ld % 8 != 0 || !host_aligned(qkv, 16) || !host_aligned(q_out, 16) || !host_aligned(rope, 16) ||
+        !host_aligned(k_codes, 16) || !host_aligned(v_codes, 16) || !host_aligned(q_weight, 16) || !host_aligned(k_weight, 16))
         return MOMIJ_ERR_INVALID_ARGUMENT;
     if (workspace && workspace_bytes < kAttnHeader) return MOMIJ_ERR_WORKSPACE;
     AppendArgs a{};
@@ -442,8 +514,9 @@ extern "C" int momij_qk_norm_rope_append(const void* qkv, long long ld, void* q_
     a.longest = longest;
     a.touched = (longest + kPage - 2) / kPage + 1;  // pages a sequence's new tokens can touch
     const long long kv = (long long)B * a.touched * Hkv * 2;
-    const int rows = kWarps * (128 / D) * kQRows;
-    const long long blocks = kv + ((long long)T * Hq + rows - 1) / rows;
+    const int heads = (256 / D) * kQRows;  // of one token, per warp
+    a.q_chunks = (Hq + heads - 1) / heads;
+    const long long blocks = kv + ((long long)T * a.q_chunks + kWarps - 1) / kWarps;
     if (blocks > 0x7fffffffLL) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     a.kv_blocks = (int)kv;
     const dim3 grid((unsigned)blocks), block(kThreads);
@@ -464,7 +537,7 @@ extern "C" int momij_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, 
     if (Hkv < 1 || (D != 64 && D != 128)) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     if (B == 0 || count == 0) return MOMIJ_OK;
     if (!k_codes || !v_codes || !k_scales || !v_scales || !block_table || !lens || !k_out || !v_out) return MOMIJ_ERR_INVALID_ARGUMENT;
-    if (!host_aligned(k_codes, 16) || !host_aligned(v_codes, 16) || !host_aligned(k_out, 8) || !host_aligned(v_out, 8))
+    if (!host_aligned(k_codes, 16) || !host_aligned(v_codes, 16) || !host_aligned(k_out, 16) || !host_aligned(v_out, 16))
         return MOMIJ_ERR_INVALID_ARGUMENT;
     if (workspace && workspace_bytes < kAttnHeader) return MOMIJ_ERR_WORKSPACE;
     ReadArgs a{};
