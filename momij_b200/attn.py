@@ -22,24 +22,37 @@ raise ``TypeError`` / ``ValueError`` before anything is enqueued.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
+import os
 from dataclasses import dataclass
 
 import torch
 
 from . import moe
-from .moe import _check, _dtype_code, lib
+from .moe import _check, lib
 
 PAGE = 64  # MOMIJ_KV_PAGE
 HEADER_BYTES = 256
 
-_vp, _i, _f, _sz, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_longlong
-lib.momij_qk_norm_rope_append.argtypes = ([_vp, _ll, _vp, _vp, _vp, _f, _vp, _i, _i, _i] + [_vp] * 4 + [_i, _vp, _i, _vp, _vp]
-                                          + [_i] * 7 + [_vp, _sz, _vp])
-lib.momij_cache_read.argtypes = [_vp] * 4 + [_i, _vp, _i, _vp, _vp, _i, _vp, _vp] + [_i] * 4 + [_vp, _sz, _vp]
-lib.momij_attention_workspace_size.argtypes = [_i, _i]
-lib.momij_attention_workspace_size.restype = _sz
-lib.momij_attention.argtypes = ([_vp, _ll, _vp, _ll] + [_vp] * 4 + [_i, _vp, _i, _vp, _vp] + [_i] * 6 + [_f, _i, _i]
-                                + [_vp, _sz, _vp])
+lib.momij_attention_workspace_size.argtypes = [ctypes.c_int, ctypes.c_int]
+lib.momij_attention_workspace_size.restype = ctypes.c_size_t
+
+
+def _load_ops():
+    """csrc/bind.cpp's module, given the addresses of this process's library."""
+    path = os.path.join(moe.HERE, "lib", "_momij_ops.so")
+    if not os.path.exists(path):
+        raise ImportError(f"{path} is missing: build it with `python -m momij_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("_momij_ops", path)
+    ops = importlib.util.module_from_spec(importlib.util.spec_from_loader("_momij_ops", loader))
+    loader.exec_module(ops)
+    ops.bind(_check, *(ctypes.cast(f, ctypes.c_void_p).value for f in (
+        lib.momij_qk_norm_rope_append, lib.momij_cache_read, lib.momij_attention, lib.momij_qmm4, lib.momij_process_logits)))
+    return ops
+
+
+_ops = _load_ops()
 
 
 @dataclass(frozen=True)
@@ -66,9 +79,6 @@ class KVCache:
                 raise ValueError("a cache lies on one CUDA device")
             if not t.is_contiguous():
                 raise ValueError("cache tensors must be contiguous")
-        ptrs = (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr())
-        object.__setattr__(self, "_ptrs", ptrs)
-        object.__setattr__(self, "_dims", (P, H, D, self.k.device))
 
 
 def new_kv_cache(n_pages: int, n_kv_heads: int, head_dim: int, device=None) -> KVCache:
@@ -98,44 +108,14 @@ def new_workspace(n_tokens: int, n_heads: int, head_dim: int = 128, device=None)
     return torch.zeros(max(workspace_size(n_tokens, n_heads), HEADER_BYTES), dtype=torch.uint8, device=device or "cuda")
 
 
-def _on(device: torch.device, *tensors) -> int:
-    """Refuses tensors on another device than the current one; its index."""
-    cur = torch.cuda.current_device()
-    if device.index != cur:
-        raise ValueError(f"tensors on {device}, current device cuda:{cur}")
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors on {t.device} and {device}")
-    return cur
-
-
-def _raw_stream(stream, index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index) if stream is None else moe._stream(stream)
-
-
-def _ints(t: torch.Tensor | None, name: str, shape) -> int | None:
-    if t is None:
-        return None
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name} is int32")
-    if tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} is a contiguous tensor of shape {shape}")
-    return t.data_ptr()
-
-
-def _table(block_table: torch.Tensor, B: int) -> int:
-    if block_table.dtype != torch.int32:
-        raise TypeError("block_table is int32")
-    if block_table.dim() != 2 or block_table.shape[0] != B or not block_table.is_contiguous():
-        raise ValueError("block_table is a contiguous [B, columns] tensor")
-    return block_table.data_ptr()
-
-
-def _keep(t: torch.Tensor, stream) -> None:
-    """A tensor allocated here and used on a stream given by the caller stays
-    allocated until that stream is done with it."""
+def _given(stream, *results):
+    """What a call on a stream of the caller's needs: its handle, and results
+    allocated on the current stream held until that stream is done with them."""
     if isinstance(stream, torch.cuda.Stream):
-        t.record_stream(stream)
+        for t in results:
+            t.record_stream(stream)
+        return stream.cuda_stream
+    return None if stream is None else int(stream)
 
 
 def qk_norm_rope_append(qkv: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, *, n_heads: int,
@@ -146,54 +126,23 @@ def qk_norm_rope_append(qkv: torch.Tensor, cache: KVCache, block_table: torch.Te
     """Norms queries and keys per head, rotates them by position and appends keys
     and values to the cache (momij_qk_norm_rope_append).  ``qkv`` [T, (Hq + 2 Hkv) D]
     (rows may be strided); returns the queries [T, Hq, D]."""
-    P, Hkv, D, dev = cache._dims
-    index = _on(dev, qkv, block_table, lens, q_weight, k_weight, rope, cu_q, q_out, workspace)
-    T, width = qkv.shape
-    B = lens.shape[0]
-    if width != (n_heads + 2 * Hkv) * D or (T > 1 and qkv.stride(0) < width) or qkv.stride(1) != 1:
-        raise ValueError(f"qkv is [T, {(n_heads + 2 * Hkv) * D}] with contiguous rows")
-    for w in (q_weight, k_weight):
-        if w is not None and (w.dtype != qkv.dtype or tuple(w.shape) != (D,) or not w.is_contiguous()):
-            raise ValueError(f"norm weights are contiguous [{D}] of the activations' dtype")
-    rows = rot = 0
-    if rope is not None:
-        rows, rot = rope.shape
-        if rope.dtype != torch.float32 or not rope.is_contiguous():
-            raise ValueError("rope is a contiguous float32 table")
-    if q_out is None:
-        q_out = torch.empty(T, n_heads, D, dtype=qkv.dtype, device=dev)
-        _keep(q_out, stream)
-    elif tuple(q_out.shape) != (T, n_heads, D) or q_out.dtype != qkv.dtype or not q_out.is_contiguous():
-        raise ValueError("q_out is a contiguous [T, Hq, D] tensor of the activations' dtype")
-    k, v, ks, vs = cache._ptrs
-    _check(lib.momij_qk_norm_rope_append(
-        qkv.data_ptr(), qkv.stride(0) if T > 1 else width, q_out.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
-        None if k_weight is None else k_weight.data_ptr(), eps, None if rope is None else rope.data_ptr(), rows, rot,
-        interleaved, k, v, ks, vs, P, _table(block_table, B), block_table.shape[1], _ints(lens, "lens", (B,)),
-        _ints(cu_q, "cu_q", (B + 1,)), T, B, max_q, n_heads, Hkv, D, _dtype_code(qkv),
-        None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes,
-        _raw_stream(stream, index)), "qkNormRopeAppend")
-    return q_out
+    if stream is not None and q_out is None:
+        q_out = torch.empty(qkv.shape[0], n_heads, cache.k.shape[3], dtype=qkv.dtype, device=qkv.device)
+    return _ops.append(qkv, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lens, n_heads, q_weight, k_weight, eps,
+                       rope, interleaved, cu_q, max_q, q_out, workspace, None if stream is None else _given(stream, q_out))
 
 
 def cache_read(cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, *, count: int, first: torch.Tensor | None = None,
                dtype=torch.bfloat16, workspace: torch.Tensor | None = None, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of ``count`` tokens per sequence from ``first[b]`` on (default 0),
     [B, count, Hkv, D]; zeros at and past ``lens[b]``."""
-    P, Hkv, D, dev = cache._dims
-    index = _on(dev, block_table, lens, first, workspace)
-    B = lens.shape[0]
-    k_out = torch.empty(B, count, Hkv, D, dtype=dtype, device=dev)
-    v_out = torch.empty(B, count, Hkv, D, dtype=dtype, device=dev)
-    _keep(k_out, stream)
-    _keep(v_out, stream)
-    k, v, ks, vs = cache._ptrs
-    _check(lib.momij_cache_read(
-        k, v, ks, vs, P, _table(block_table, B), block_table.shape[1], _ints(lens, "lens", (B,)), _ints(first, "first", (B,)),
-        count, k_out.data_ptr(), v_out.data_ptr(), B, Hkv, D, _dtype_code(k_out),
-        None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes,
-        _raw_stream(stream, index)), "cacheRead")
-    return k_out, v_out
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"values are bf16 or fp16, not {dtype}")
+    out = _ops.read(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lens, first, count, dtype == torch.float16,
+                    workspace, None if stream is None else _given(stream))
+    if stream is not None:
+        _given(stream, *out)
+    return out
 
 
 def attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, *, scale: float | None = None,
@@ -202,24 +151,10 @@ def attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens: 
     """Causal attention of the new tokens' queries ``q`` [T, Hq, D] over the cache
     (momij_attention); ``scale`` defaults to D^-1/2, ``window`` 0 means all positions.
     Token rows of ``q`` and ``out`` may be strided."""
-    P, Hkv, D, dev = cache._dims
-    index = _on(dev, q, block_table, lens, cu_q, out, workspace)
-    T, Hq, d = q.shape
-    B = lens.shape[0]
-    if d != D or q.stride(2) != 1 or (Hq > 1 and q.stride(1) != D):
-        raise ValueError(f"q is [T, Hq, {D}] with contiguous rows")
-    if out is None:
-        out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
-        _keep(out, stream)
-    elif tuple(out.shape) != (T, Hq, D) or out.dtype != q.dtype or out.stride(2) != 1 or (Hq > 1 and out.stride(1) != D):
-        raise ValueError("out is [T, Hq, D] of q's dtype with contiguous rows")
     if workspace is None:
-        workspace = new_workspace(T, Hq, D, dev)
-        _keep(workspace, stream)
-    k, v, ks, vs = cache._ptrs
-    _check(lib.momij_attention(
-        q.data_ptr(), q.stride(0) if T > 1 else Hq * D, out.data_ptr(), out.stride(0) if T > 1 else Hq * D, k, v, ks, vs, P,
-        _table(block_table, B), block_table.shape[1], _ints(lens, "lens", (B,)), _ints(cu_q, "cu_q", (B + 1,)), T, B, max_q,
-        Hq, Hkv, D, D ** -0.5 if scale is None else scale, window, _dtype_code(q), workspace.data_ptr(), workspace.nbytes,
-        _raw_stream(stream, index)), "attention")
-    return out
+        workspace = new_workspace(q.shape[0], q.shape[1], device=q.device)
+        _given(stream, workspace)
+    if stream is not None and out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    return _ops.attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lens, scale, window, cu_q, max_q, out,
+                          workspace, None if stream is None else _given(stream, out))

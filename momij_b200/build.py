@@ -1,4 +1,5 @@
-"""Builds libmomij_moe.so in-tree (momij_b200/lib/) for sm_100a with nvcc.
+"""Builds libmomij_moe.so in-tree (momij_b200/lib/) for sm_100a with nvcc, and
+_momij_ops.so beside it (the Python entry of the attn and head operators).
 
 Each .cu under csrc/ is compiled separately (parallel), then linked into one
 shared library with the CUDA runtime linked statically, so the library does
@@ -59,11 +60,37 @@ def _compile(src: str, verbose_ptxas: bool) -> str:
     return out
 
 
+def _bind() -> str:
+    """_momij_ops.so: the Python entry of the attn and head operators (a CPython
+    module over torch's tensors; libmomij_moe.so itself needs neither)."""
+    import sysconfig
+
+    import torch
+    src = os.path.join(CSRC, "bind.cpp")
+    out = os.path.join(LIB_DIR, "_momij_ops.so")
+    deps = [src, os.path.join(ROOT, "include", "momij_moe.h")]
+    if os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(d) for d in deps):
+        return out
+    inc, lib = os.path.join(os.path.dirname(torch.__file__), "include"), os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    cmd = ["/usr/bin/g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", src, "-o", out,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
+           "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"),
+           "-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for bind.cpp:\n{r.stderr}")
+    return out
+
+
 def build(jobs: int = 4, verbose_ptxas: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        bound = ex.submit(_bind)
         objs = list(ex.map(lambda s: _compile(s, verbose_ptxas), SOURCES))
+        bound.result()
     if (not os.path.exists(LIB) or
             os.path.getmtime(LIB) < max(os.path.getmtime(o) for o in objs)):
         cmd = [nvcc()] + ARCH + ["-shared", "-o", LIB] + objs + ["-cudart", "static", "-ldl",
