@@ -286,18 +286,15 @@ __global__ void __launch_bounds__(Shape<NB>::kWarps * 32, 1) attn_kernel(const A
             }
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // the row's largest magnitude becomes 2^13 .. 2^14 (zeros, infinities and NaN: left)
-            const uint32_t tb = __float_as_uint(Half<DT>::to_f((uint16_t)top));
-            const int sh = tb != 0 && tb < 0x7f800000u ? 13 - ilogbf(__uint_as_float(tb)) : 0;
-            const float f0 = ldexpf(1.f, sh / 2), f1 = ldexpf(1.f, sh - sh / 2);  // two steps: 2^sh can leave fp32
+            const RowScale rs = row_scale(Half<DT>::to_f((uint16_t)top));
 #pragma unroll
             for (int i = 0; i < D / 64; ++i)
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    f[i * 4 + w][0] = f16x2(e[i][4 * w] * f0 * f1, e[i][4 * w + 1] * f0 * f1);
-                    f[i * 4 + w][1] = f16x2(e[i][4 * w + 2] * f0 * f1, e[i][4 * w + 3] * f0 * f1);
+                    f[i * 4 + w][0] = f16x2(e[i][4 * w] * rs.up, e[i][4 * w + 1] * rs.up);
+                    f[i * 4 + w][1] = f16x2(e[i][4 * w + 2] * rs.up, e[i][4 * w + 3] * rs.up);
                 }
-            return ldexpf(a.scale_log2, -sh);
+            return a.scale_log2 * rs.down;
         };
         if (kSharedQ) {
             if (warp < NB) {
@@ -531,7 +528,7 @@ __global__ void __launch_bounds__(Shape<NB>::kWarps * 32, 1) attn_kernel(const A
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                unsigned* ctr = a.counters + ((long long)(sq.t0 * a.G + row0) * a.Hkv + h);
+                unsigned* ctr = a.counters + cf;
                 const unsigned old = atomicAdd(ctr, 1u);
                 s_last = old == (unsigned)(cl - cf);
                 if (s_last) *ctr = 0u;
@@ -608,8 +605,14 @@ int launch_rows(const AttnArgs& a, int rows, int grid, momij_stream_t st) {
     return launch<DT, D, 4>(a, grid, st);
 }
 
-size_t part_bytes(int sms) { return (size_t)2 * sms * (kMaxRows * 128 + 2 * kMaxRows) * 4; }
-size_t counter_bytes(long long rows) { return ((size_t)rows * 4 + 255) / 256 * 256; }
+// Room for the partial results of calls of up to `rows` (token, head) rows.
+size_t part_bytes(int sms, long long rows) {
+    const size_t few = (size_t)2 * sms * (kMaxRows * 128 + 2 * kMaxRows) * 4;
+    return rows < kPrefillRows ? few : std::max(few, attn_prefill_part_bytes(sms));
+}
+// One counter per block, at a fixed place: a segment that blocks share counts
+// with its first block's, and a block is the first of one such segment at most.
+constexpr size_t kCounterBytes = 4096;
 
 }  // namespace
 }  // namespace momij
@@ -620,7 +623,7 @@ extern "C" size_t momij_attention_workspace_size(int T, int Hq) {
     if (T < 0 || Hq < 0) return 0;
     int sms = host_sm_count();
     if (sms <= 0) sms = 148;  // without a device: a B200's
-    return kAttnHeader + counter_bytes((long long)T * Hq) + part_bytes(sms);
+    return kAttnHeader + kCounterBytes + part_bytes(sms, (long long)T * Hq);
 }
 
 extern "C" int momij_attention(const void* q, long long ldq, void* out, long long ldo, const uint8_t* k_codes, const uint8_t* v_codes,
@@ -641,7 +644,7 @@ extern "C" int momij_attention(const void* q, long long ldq, void* out, long lon
         return MOMIJ_ERR_INVALID_ARGUMENT;
     if ((long long)T * Hq > (1LL << 30)) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     const int sms = host_sm_count();
-    if (sms <= 0) return MOMIJ_ERR_CUDA;
+    if (sms <= 0 || sms > (int)(kCounterBytes / 4)) return MOMIJ_ERR_CUDA;
     if (workspace_bytes < momij_attention_workspace_size(T, Hq)) return MOMIJ_ERR_WORKSPACE;
 
     AttnArgs a{};
@@ -656,10 +659,8 @@ extern "C" int momij_attention(const void* q, long long ldq, void* out, long lon
     a.cu = cu_q;
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     a.ws = reinterpret_cast<int32_t*>(ws);
-    // the partial results first: their place does not depend on the call's sizes,
-    // so a smaller call's counters are never where a larger one left results
-    a.parts = reinterpret_cast<float*>(ws + kAttnHeader);
-    a.counters = reinterpret_cast<unsigned*>(ws + kAttnHeader + part_bytes(sms));
+    a.counters = reinterpret_cast<unsigned*>(ws + kAttnHeader);
+    a.parts = reinterpret_cast<float*>(ws + kAttnHeader + kCounterBytes);
     a.stop = host_stop_flag();
     a.ldq = ldq;
     a.ldo = ldo;
@@ -676,6 +677,7 @@ extern "C" int momij_attention(const void* q, long long ldq, void* out, long lon
     a.spin = host_spin_limit();
     a.scale_log2 = scale * 1.4426950408889634f;
     const long long rows = (long long)a.longest * a.G;
+    if (rows >= kPrefillRows) return attn_prefill_launch(a, D, dtype, sms, stream);
     const int rb = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     const long long nrb = (rows + rb - 1) / rb;
     // sequences per launch: their row blocks and units (row block, head, page) stay countable

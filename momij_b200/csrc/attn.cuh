@@ -12,7 +12,7 @@ struct AttnArgs {
     const float *ks, *vs;
     const int32_t *table, *lens, *cu;
     int32_t* ws;         // header words
-    unsigned* counters;  // one per query row and head, zero between calls
+    unsigned* counters;  // one per block, zero between calls
     float* parts;        // partial results of segments that several blocks share
     const int32_t* stop;
     long long ldq, ldo;
@@ -52,6 +52,22 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-int attn_prefill_launch(const AttnArgs& a, int D, int dtype, int max_q, momij_stream_t st);
+// The power of two that brings a row's largest magnitude to 2^13 .. 2^14, and
+// its inverse, from the exponent alone; 1 for zeros, infinities and NaN.  Rows
+// whose largest magnitude is below 2^-113 stay smaller (their scores are nil).
+struct RowScale {
+    float up, down;
+};
+__device__ __forceinline__ RowScale row_scale(float top) {
+    const uint32_t u = __float_as_uint(top);
+    if (u == 0u || u >= 0x7f800000u) return {1.f, 1.f};
+    const int e = max((int)(u >> 23), 14);
+    return {__uint_as_float((uint32_t)(267 - e) << 23), __uint_as_float((uint32_t)(e - 13) << 23)};
+}
+
+// Rows per sequence from which attention goes to attn_prefill.cu.
+constexpr int kPrefillRows = 128;
+int attn_prefill_launch(const AttnArgs& a, int D, int dtype, int sms, momij_stream_t st);
+size_t attn_prefill_part_bytes(int sms);
 
 }  // namespace momij
