@@ -17,7 +17,7 @@
 // power of two, which holds bf16's 8 bits exactly.
 //
 // Work.  A cache read once is all that a decode step needs, so the heads of a
-// group and the drafted tokens share it: a row block is 8, 16 or 32 (token,
+// group and the drafted tokens share it: a row block is 8 or 16 (token,
 // head) rows of one sequence and one kv head, multiplied by mma.sync m16n8k16
 // with the cache's codes as the 16-row operand (tokens for the scores,
 // dimensions for the outputs) and the rows as its 8 columns: a decode step's
@@ -43,7 +43,9 @@ namespace {
 
 constexpr int kMaxSeg = 4096;   // row blocks per launch (their prefix sums live in shared memory)
 constexpr int kMinPages = 4;    // pages per block at least, unless the segments are shorter
-constexpr int kMaxRows = 32;    // rows of a row block at most
+constexpr int kMaxRows = 16;    // rows of a row block at most
+constexpr int kWarps = 12, kThreads = kWarps * 32;
+constexpr int kStages = 2;      // of a warp's ring
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -82,28 +84,18 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const AttnSeq& s, int
     return p;
 }
 
-template <int NB>
-struct Shape {  // of a block: warps and stages of their rings, by rows per block (8 NB)
-    static constexpr int kWarps = NB == 4 ? 8 : 12;
-    static constexpr int kStages = NB == 4 ? 3 : 2;
-};
-
 template <int DT, int D, int NB>
-__global__ void __launch_bounds__(Shape<NB>::kWarps * 32, 1) attn_kernel(const AttnArgs a) {
-    constexpr int kWarps = Shape<NB>::kWarps, kThreads = kWarps * 32, kStages = Shape<NB>::kStages;
+__global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
     constexpr int RB = 8 * NB, KS = D / 16, MD = D / 16;
     constexpr int kKBytes = 32 * D, kStage = 2 * kKBytes;  // a half page of K and of V
     constexpr int kOPitch = D + 4;
-    constexpr bool kSharedQ = NB == 4;  // q fragments in shared memory rather than registers
     extern __shared__ __align__(16) unsigned char smem[];
-    // [stages of all warps, then their results] [q fragments, row factors] [warp maxima and sums] [prefix]
+    // [stages of all warps, then their results] [warp maxima and sums] [prefix]
     float* s_o = reinterpret_cast<float*>(smem);
     constexpr int kRing = kWarps * kStages * kStage;
     constexpr int kJoin = kWarps * RB * kOPitch * 4;
     constexpr int kArea = kRing > kJoin ? kRing : kJoin;
-    uint2* s_q = reinterpret_cast<uint2*>(smem + kArea);
-    float* s_fac = reinterpret_cast<float*>(smem + kArea + (kSharedQ ? KS * NB * 256 : 0));
-    float* s_m = s_fac + RB;
+    float* s_m = reinterpret_cast<float*>(smem + kArea);
     float* s_l = s_m + kWarps * RB;
     int* s_pref = reinterpret_cast<int*>(s_l + kWarps * RB);
     __shared__ int s_scan[kWarps], s_full[kWarps];
@@ -255,9 +247,9 @@ __global__ void __launch_bounds__(Shape<NB>::kWarps * 32, 1) attn_kernel(const A
 
         // ---- q as fp16 fragments: lane (g, c) holds, for row g of each 8, the
         // 16 elements from 64 i + 16 c on ------------------------------------------
-        uint32_t qf[kSharedQ ? 1 : NB][KS][2];
-        float fac[NB][2];
-        auto load_q = [&](int nb, uint32_t (&f)[KS][2]) -> float {
+        uint32_t qf[NB][KS][2];
+        float fac[NB][2], shift[NB][2];  // per row 2c, 2c + 1: factor of the scores, and what the codes' offset adds to them
+        auto load_q = [&](int nb, uint32_t (&f)[KS][2]) -> float2 {
             const int r = 8 * nb + g, row = row0 + r;
             float e[D / 64][16];
             uint32_t top = 0;
@@ -287,35 +279,29 @@ __global__ void __launch_bounds__(Shape<NB>::kWarps * 32, 1) attn_kernel(const A
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const RowScale rs = row_scale(Half<DT>::to_f((uint16_t)top));
+            float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < D / 64; ++i)
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    f[i * 4 + w][0] = f16x2(e[i][4 * w] * rs.up, e[i][4 * w + 1] * rs.up);
-                    f[i * 4 + w][1] = f16x2(e[i][4 * w + 2] * rs.up, e[i][4 * w + 3] * rs.up);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t h = f16x2(e[i][4 * w + 2 * k] * rs.up, e[i][4 * w + 2 * k + 1] * rs.up);
+                        f[i * 4 + w][k] = h;
+                        sum += Half<MOMIJ_DTYPE_F16>::to_f((uint16_t)(h & 0xffffu)) + Half<MOMIJ_DTYPE_F16>::to_f((uint16_t)(h >> 16));
+                    }
                 }
-            return a.scale_log2 * rs.down;
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            return make_float2(a.scale_log2 * rs.down * kRawUnit, -kRawOffset / kRawUnit * sum);
         };
-        if (kSharedQ) {
-            if (warp < NB) {
-                uint32_t f[KS][2];
-                const float v = load_q(warp, f);
 #pragma unroll
-                for (int k = 0; k < KS; ++k) s_q[(k * NB + warp) * 32 + lane] = make_uint2(f[k][0], f[k][1]);
-                if (c == 0) s_fac[8 * warp + g] = v;
-            }
-            __syncthreads();
+        for (int nb = 0; nb < NB; ++nb) {
+            const float2 v = load_q(nb, qf[nb]);
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                fac[nb][0] = s_fac[8 * nb + 2 * c];
-                fac[nb][1] = s_fac[8 * nb + 2 * c + 1];
-            }
-        } else {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const float v = load_q(nb, qf[kSharedQ ? 0 : nb]);
-                fac[nb][0] = __shfl_sync(0xffffffffu, v, 8 * c);
-                fac[nb][1] = __shfl_sync(0xffffffffu, v, 8 * c + 4);
+            for (int e = 0; e < 2; ++e) {
+                fac[nb][e] = __shfl_sync(0xffffffffu, v.x, 8 * c + 4 * e);
+                shift[nb][e] = __shfl_sync(0xffffffffu, v.y, 8 * c + 4 * e);
             }
         }
 
@@ -366,30 +352,28 @@ __global__ void __launch_bounds__(Shape<NB>::kWarps * 32, 1) attn_kernel(const A
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const uint32_t word = w == 0 ? kw[q].x : w == 1 ? kw[q].y : w == 2 ? kw[q].z : kw[q].w;
-                        lo[q] = codes_f16x2(word, 0x4140);
-                        hi[q] = codes_f16x2(word, 0x4342);
+                        lo[q] = codes_raw(word, 0x4140);
+                        hi[q] = codes_raw(word, 0x4342);
                     }
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        uint2 qb;
-                        if (kSharedQ) qb = s_q[((i * 4 + w) * NB + nb) * 32 + lane];
-                        else qb = make_uint2(qf[kSharedQ ? 0 : nb][i * 4 + w][0], qf[kSharedQ ? 0 : nb][i * 4 + w][1]);
-                        mma_f16(s[nb][0], lo[0], lo[1], hi[0], hi[1], qb.x, qb.y);
-                        mma_f16(s[nb][1], lo[2], lo[3], hi[2], hi[3], qb.x, qb.y);
+                        mma_f16(s[nb][0], lo[0], lo[1], hi[0], hi[1], qf[nb][i * 4 + w][0], qf[nb][i * 4 + w][1]);
+                        mma_f16(s[nb][1], lo[2], lo[3], hi[2], hi[3], qf[nb][i * 4 + w][0], qf[nb][i * 4 + w][1]);
                     }
                 }
             }
-            // weights: x = fac ks (q.c) + log2 vs; a page of zeros (scale 0) keeps its weight in the sum
+            // weights: x = fac ks (q.c - 128 sum q) + log2 vs; a page of zeros (scale 0) keeps its weight in the sum
             const float lv = vs == 0.f ? 0.f : __log2f(vs), iv = vs == 0.f ? 1.f : __fdividef(1.f, vs);
             const bool inside = t0 + 32 <= all_hi && t0 >= all_lo;
             uint32_t p[NB][4];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const float al[2] = {fac[nb][0] * ks, fac[nb][1] * ks};
+                const float base[2] = {fmaf(shift[nb][0], al[0], lv), fmaf(shift[nb][1], al[1], lv)};
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[nb][t][e] = fmaf(s[nb][t][e], al[e & 1], lv);
+                    for (int e = 0; e < 4; ++e) s[nb][t][e] = fmaf(s[nb][t][e], al[e & 1], base[e & 1]);
                 if (!inside) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -590,19 +574,16 @@ __global__ void __launch_bounds__(Shape<NB>::kWarps * 32, 1) attn_kernel(const A
 
 template <int DT, int D, int NB>
 int launch(const AttnArgs& a, int grid, momij_stream_t st) {
-    constexpr int RB = 8 * NB, W = Shape<NB>::kWarps;
-    constexpr size_t ring = (size_t)W * Shape<NB>::kStages * 64 * D, join = (size_t)W * RB * (D + 4) * 4;
-    const size_t smem = (ring > join ? ring : join) + (NB == 4 ? (D / 16) * NB * 256 : 0) + RB * 4 + 2 * W * RB * 4 +
-                        ((size_t)a.nb * a.nrb + 1) * 4;
+    constexpr int RB = 8 * NB;
+    constexpr size_t ring = (size_t)kWarps * kStages * 64 * D, join = (size_t)kWarps * RB * (D + 4) * 4;
+    const size_t smem = (ring > join ? ring : join) + 2 * kWarps * RB * 4 + ((size_t)a.nb * a.nrb + 1) * 4;
     static int granted[64];
     if (!host_allow_smem(attn_kernel<DT, D, NB>, smem, granted)) return MOMIJ_ERR_CUDA;
-    return host_launch(attn_kernel<DT, D, NB>, dim3(grid), dim3(W * 32), smem, st, a);
+    return host_launch(attn_kernel<DT, D, NB>, dim3(grid), dim3(kThreads), smem, st, a);
 }
 template <int DT, int D>
 int launch_rows(const AttnArgs& a, int rows, int grid, momij_stream_t st) {
-    if (rows == 8) return launch<DT, D, 1>(a, grid, st);
-    if (rows == 16) return launch<DT, D, 2>(a, grid, st);
-    return launch<DT, D, 4>(a, grid, st);
+    return rows == 8 ? launch<DT, D, 1>(a, grid, st) : launch<DT, D, 2>(a, grid, st);
 }
 
 // Room for the partial results of calls of up to `rows` (token, head) rows.
@@ -678,8 +659,8 @@ extern "C" int momij_attention(const void* q, long long ldq, void* out, long lon
     a.scale_log2 = scale * 1.4426950408889634f;
     const long long rows = (long long)a.longest * a.G;
     if (rows >= kPrefillRows) return attn_prefill_launch(a, D, dtype, sms, stream);
-    const int rb = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-    const long long nrb = (rows + rb - 1) / rb;
+    const int rb = rows <= 8 ? 8 : 16;
+    const long long nrb = (rows + rb - 1) / rb;  // (1: more rows go to tcgen05)
     // sequences per launch: their row blocks and units (row block, head, page) stay countable
     const long long units = nrb * Hkv * std::max(table_cols, 1);
     if (nrb > kMaxSeg || units > (1LL << 30)) return MOMIJ_ERR_UNSUPPORTED_SHAPE;

@@ -65,8 +65,13 @@ __device__ __forceinline__ RowScale row_scale(float top) {
     return {__uint_as_float((uint32_t)(267 - e) << 23), __uint_as_float((uint32_t)(e - 13) << 23)};
 }
 
-// Rows per sequence from which attention goes to attn_prefill.cu.
-constexpr int kPrefillRows = 128;
+// Rows (tokens times heads of a group) per sequence from which attention goes
+// to attn_prefill.cu.  Measured, us for 16 / 24 / 32 rows, attn.cu's kernel (row
+// blocks of 16 and 32) against that one's: 24 sequences of 5,003 tokens, 4 kv
+// heads of 128: 46.8 / 60.0 / 62.5 against 64.2 / 64.4 / 64.5; one of 30,000, 2 of
+// 128: 31.9 / 42.5 / 49.9 against 26.0 / 25.9 / 26.3; 4 of 2,000, 8 of 128: 20.4 /
+// 24.7 / 26.0 against 17.5 / 17.8 / 18.0.
+constexpr int kPrefillRows = 17;
 int attn_prefill_launch(const AttnArgs& a, int D, int dtype, int sms, momij_stream_t st);
 size_t attn_prefill_part_bytes(int sms);
 

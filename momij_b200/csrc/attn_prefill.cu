@@ -305,16 +305,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
                                              (i % (KL / 2)) * 256 + ct);
             }
         };
-        // sixteen codes as 32 bytes of fp16 at chunks c, c + 1 of row r (`swap`: the second first)
-        auto store = [&](uint32_t atom, int r, int c, bool swap, const uint4& v) {
+        // sixteen codes as 32 bytes of fp16 at chunks c, c + 1 of row r: K's as c * 2^-24,
+        // V's as signed integers (`swap`: the second chunk first)
+        auto store = [&](uint32_t atom, int r, int c, bool swap, bool raw, const uint4& v) {
             const uint32_t row = atom + (r >> 3) * 1024 + (r & 7) * 128;
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int q = swap ? 1 - e : e;
                 const uint32_t x = q ? w[2] : w[0], y = q ? w[3] : w[1];
-                sts16(row + (((c + q) ^ (r & 7)) << 4), codes_f16x2(x, 0x4140), codes_f16x2(x, 0x4342), codes_f16x2(y, 0x4140),
-                      codes_f16x2(y, 0x4342));
+                const uint32_t to = row + (((c + q) ^ (r & 7)) << 4);
+                if (raw) sts16(to, codes_raw(x, 0x4140), codes_raw(x, 0x4342), codes_raw(y, 0x4140), codes_raw(y, 0x4342));
+                else sts16(to, codes_f16x2(x, 0x4140), codes_f16x2(x, 0x4342), codes_f16x2(y, 0x4140), codes_f16x2(y, 0x4342));
             }
         };
         if (J > 0) {
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             for (int i = 0; i < KL; ++i) {
                 const int ci = (i % (KL / 2)) * 256 + ct, r = ci / CPR + (i / (KL / 2)) * kPage, ch = ci % CPR;
                 // 64 elements an atom; lanes of the second atom store their halves the other way round (banks)
-                store(kt + (ch >> 2) * (kTileK * 128), r, (ch & 3) * 2, D == 128 && (ch & 4), kr[i]);
+                store(kt + (ch >> 2) * (kTileK * 128), r, (ch & 3) * 2, D == 128 && (ch & 4), true, kr[i]);
             }
             fence_async();
             mbar_arrive(&b_kfull[st]);
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
 #pragma unroll
             for (int i = 0; i < KL; ++i) {
                 const int ci = (i % (KL / 2)) * 256 + ct;  // row d = ci / 4, 16 tokens of the page
-                store(vt + (i / (KL / 2)) * (D * 128), ci >> 2, (ci & 3) * 2, false, vr[i]);
+                store(vt + (i / (KL / 2)) * (D * 128), ci >> 2, (ci & 3) * 2, false, false, vr[i]);
             }
             fence_async();
             mbar_arrive(&b_vfull[st]);
@@ -391,18 +393,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             }
             const RowScale rs = row_scale(Half<DT>::to_f((uint16_t)top));
             const float f0 = pa.negate ? -rs.up : rs.up;
-            const float fac = a.scale_log2 * rs.down;
+            const float fac = a.scale_log2 * rs.down * kRawUnit;
+            float qsum = 0.f;  // of the row as rounded, for the codes' offset
             const uint32_t qt = base + SM::kQ;
 #pragma unroll 4
-            for (int c = e * (D / 16); c < (e + 1) * (D / 16); ++c) {
+            for (int c = 0; c < D / 8; ++c) {
                 const uint4 v = load8(c);
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
                 uint32_t o[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
+                for (int k = 0; k < 4; ++k) {
                     o[k] = f16x2(Half<DT>::to_f((uint16_t)(w[k] & 0xffffu)) * f0, Half<DT>::to_f((uint16_t)(w[k] >> 16)) * f0);
-                sts16(qt + (c >> 3) * (kTileQ * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+                    qsum += Half<MOMIJ_DTYPE_F16>::to_f((uint16_t)(o[k] & 0xffffu)) + Half<MOMIJ_DTYPE_F16>::to_f((uint16_t)(o[k] >> 16));
+                }
+                if (c / (D / 16) == e)
+                    sts16(qt + (c >> 3) * (kTileQ * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
             }
+            const float shift = -kRawOffset / kRawUnit * qsum;
             fence_async();
             mbar_arrive(&b_q);
 
@@ -410,17 +417,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             // keys that every row of the tile sees
             const int all_hi = sq.past + row0 / a.G + 1;
             const int all_lo = a.window > 0 ? sq.past + (row0 + rows - 1) / a.G - a.window + 1 : 0;
+            const bool idle = (warp & 3) * 32 >= rows;
             for (int j = 0; j < J; ++j) {
                 const int st = j & 1;
                 const uint32_t ts = lanes + st * 128 + e * 64;  // this thread's 64 scores
                 ok = __all_sync(0xffffffffu, wait(&b_s[st], (j >> 1) & 1));
                 if (!ok) break;
                 tc_after_sync();
+                if (idle) {  // no row of this warp's is written
+                    tc_before_sync();
+                    mbar_arrive(&b_p[st][e]);
+                    continue;
+                }
                 float s[kPage];
                 tmem_ld32_nowait(ts, *reinterpret_cast<uint32_t(*)[32]>(s));
                 tmem_ld32_nowait(ts + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
                 const float* sc = s_scale[j & (kScaleRing - 1)][e];
-                float al = fac * sc[0], lv = sc[1];
+                float al = fac * sc[0], lv = fmaf(shift, al, sc[1]);
                 const float iv = sc[2];
                 const int t0 = (first_page + 2 * j + e) * kPage;
                 tmem_ld_wait();
@@ -597,7 +610,9 @@ int launch(const PrefillArgs& pa, int grid, momij_stream_t st) {
 
 }  // namespace
 
-size_t attn_prefill_part_bytes(int sms) { return (size_t)sms * part_floats(128) * 4; }
+// Partial results that the workspace has room for.
+static int attn_prefill_slots(int sms) { return 3 * sms; }
+size_t attn_prefill_part_bytes(int sms) { return (size_t)attn_prefill_slots(sms) * part_floats(128) * 4; }
 
 int attn_prefill_launch(const AttnArgs& a, int D, int dtype, int sms, momij_stream_t st) {
     PrefillArgs pa{};
@@ -608,9 +623,23 @@ int attn_prefill_launch(const AttnArgs& a, int D, int dtype, int sms, momij_stre
     const long long tiles = (rows + kTileQ - 1) / kTileQ, blocks = tiles * a.B * a.Hkv;
     if (blocks > 0x7fffffffLL) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     pa.tiles = (int)tiles;
-    // blocks that fit side by side share a row tile's keys, four tiles (512 keys) each at least
-    const int most = std::max(1, std::min(a.window > 0 ? (a.window + a.longest) / 512 : a.table_cols / 8, 32));
-    pa.splits = (int)std::max<long long>(1, std::min<long long>(sms / blocks, most));
+    // Blocks per row tile: with s of them the SMs work through about (blocks *
+    // (keys + s * start)) / sms tiles each, and the longest block ends up to keys / s
+    // after the others; `start` is a block's own start and end in units of tiles
+    // (about 5 us against 1.1).  The sequences' lengths are not known here: two
+    // thirds of the table's.
+    const int keys = std::max(1, (a.window > 0 ? std::min(a.window + a.longest, a.table_cols * kPage) : a.table_cols * kPage) / kTileK);
+    const long long most = std::min<long long>({(long long)attn_prefill_slots(sms) / blocks, (long long)(keys + 3) / 4, 32LL});
+    pa.splits = 1;
+    double best = 1e30;
+    for (int s = 1; s == 1 || s <= most; ++s) {
+        const double rounds = (double)blocks * (0.67 * keys + 4.5 * s) / sms, tail = (double)keys / s + 4.5;
+        const double cost = std::max(rounds, 0.67 * keys / s + 4.5) + 0.5 * tail + (s > 1 ? 2.0 : 0.0);
+        if (cost < best) {
+            best = cost;
+            pa.splits = s;
+        }
+    }
     const int grid = (int)(blocks * pa.splits);
     if (dtype == MOMIJ_DTYPE_BF16)
         return D == 64 ? launch<MOMIJ_DTYPE_BF16, 64>(pa, grid, st) : launch<MOMIJ_DTYPE_BF16, 128>(pa, grid, st);

@@ -6,9 +6,8 @@
 // A code c in 1..255 stands for (c - 128) * scale of its page and head.  A
 // page holds 64 consecutive tokens of one sequence; block_table[b, i] names
 // the page of tokens 64 i .. 64 i + 63 of sequence b.
-//   * offset codes: (c ^ 0x64 << 8) is the fp16 number 1024 + c, so a byte
-//     permute and one subtraction of 1152 make two operands of the matrix
-//     units from two codes, without a sign fix;
+//   * offset codes: one byte permute makes fp16 numbers of two codes (c * 2^-24,
+//     or 1024 + c, from which 1152 is subtracted), without a sign fix;
 //   * V transposed: the product with the weights sums over tokens, which then
 //     lie side by side like the dimensions of K do for the scores.
 #pragma once
@@ -33,5 +32,13 @@ __device__ __forceinline__ uint32_t codes_f16x2(uint32_t w, uint32_t sel) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));  // 1152
     return r;
 }
+
+// Two codes as packed fp16 subnormals c * 2^-24, exactly: one byte permute.
+// Good for the scores (q.c with c in 1 .. 255, from which 128 sum(q) goes off
+// again: a sum of D terms, three times what it is without the offset).  The
+// outputs' sums over tokens keep the signed integers: thousands of weights times
+// 128 would cancel there, and the accumulator's roundings with them.
+__device__ __forceinline__ uint32_t codes_raw(uint32_t w, uint32_t sel) { return __byte_perm(w, 0u, sel); }
+constexpr float kRawUnit = 16777216.f, kRawOffset = 128.f;
 
 }  // namespace momij
