@@ -43,6 +43,7 @@ namespace {
 
 constexpr int kMaxSeg = 4096;   // row blocks per launch (their prefix sums live in shared memory)
 constexpr int kMinPages = 4;    // pages per block at least, unless the segments are shorter
+constexpr int kStartPages = 10, kJoinPages = 8;  // what a piece's start and a join cost: about 4 and 3 us against 0.37 a page
 constexpr int kMaxRows = 16;    // rows of a row block at most
 constexpr int kWarps = 12, kThreads = kWarps * 32;
 constexpr int kStages = 2;      // of a warp's ring
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
     float* s_m = reinterpret_cast<float*>(smem + kArea);
     float* s_l = s_m + kWarps * RB;
     int* s_pref = reinterpret_cast<int*>(s_l + kWarps * RB);
-    __shared__ int s_scan[kWarps], s_full[kWarps];
+    __shared__ int s_scan[kWarps], s_full[kWarps], s_long[kWarps];
     __shared__ int s_last;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
 
     // ---- prefix sums of the segments' pages, and the segments that have any ---
     const int nseg = a.nb * a.nrb, per = (nseg + kThreads - 1) / kThreads;
-    int sum = 0, full = 0;
+    int sum = 0, full = 0, most = 0;
     for (int i = 0; i < per; ++i) {
         const int sg = tid * per + i;
         if (sg < nseg) {
@@ -118,6 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
             if (!s.ok && sg % a.nrb == 0) cache_error(a.ws, MOMIJ_ERR_PAGE);
             sum += p.hi - p.lo;
             full += p.hi > p.lo;
+            most = max(most, p.hi - p.lo);
             s_pref[sg + 1] = sum;  // within this thread's run
         }
     }
@@ -128,17 +130,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
         if (lane >= o) inc += v;
     }
     full = __reduce_add_sync(0xffffffffu, full);
+    most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 31) {
         s_scan[warp] = inc;
         s_full[warp] = full;
+        s_long[warp] = most;
     }
     __syncthreads();
-    int base = inc - sum, total = 0, nfull = 0;
+    int base = inc - sum, nfull = 0, longest = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
         if (w < warp) base += s_scan[w];
-        total += s_scan[w];
         nfull += s_full[w];
+        longest = max(longest, s_long[w]);
     }
     for (int i = 0; i < per; ++i) {
         const int sg = tid * per + i;
@@ -146,8 +150,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
     }
     if (tid == 0) s_pref[0] = 0;
     __syncthreads();
-    const int U = total * a.Hkv;  // below 2^31: the host bounds the launch
-
     // rows that see no key at all
     if (nfull < nseg)
         for (int sg = blockIdx.x; sg < nseg; sg += gridDim.x)
@@ -160,33 +162,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
                 }
             }
 
-    // Blocks in use: all of them when there is a share of kMinPages for each,
-    // fewer for short contexts, but one per (segment, head) where those are
-    // shorter still: they are independent, and a block takes one at a time.
-    const int nblk = min((int)gridDim.x, max((U + kMinPages - 1) / kMinPages, min(nfull, 1 << 20) * a.Hkv));
-    if ((int)blockIdx.x >= nblk) {
+    const Line line(s_pref, nseg, nfull, longest, a.Hkv, gridDim.x, kMinPages, kStartPages, kJoinPages);
+    if ((int)blockIdx.x >= line.blocks) {
         pdl_launch_dependents();
         return;
     }
-    const int sh_q = U / nblk, sh_r = U - sh_q * nblk;  // the first sh_r shares hold one unit more
-    auto share = [&](int i) -> int { return sh_q * i + min(i, sh_r); };
-    auto owner = [&](int x) -> int {
-        const int cut = sh_r * (sh_q + 1);
-        return x < cut ? x / (sh_q + 1) : sh_r + (x - cut) / sh_q;
-    };
-    const int u0 = share(blockIdx.x), u1 = share(blockIdx.x + 1);
-
+    int u0, u1, seg;
+    line.range(blockIdx.x, nseg, u0, u1, seg);
     int u = u0;
-    int seg = 0;
-    {  // the segment that holds u0
-        int lo = 0, hi = nseg - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (s_pref[mid] * a.Hkv <= u) lo = mid;
-            else hi = mid - 1;
-        }
-        seg = lo;
-    }
     while (u < u1) {
         while (s_pref[seg + 1] * a.Hkv <= u) ++seg;
         const int b = a.b0 + seg / a.nrb, row0 = (seg % a.nrb) * RB;
@@ -318,17 +301,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
         const int all_hi = sq.past + row0 / a.G + 1;
         const int all_lo = a.window > 0 ? sq.past + (row0 + span.rows - 1) / a.G - a.window + 1 : 0;
 
-        int slot = 0;
+        int stage = 0;
         for (int it = 0; warp + kWarps * it < n_items; ++it) {
             const float ks = sc[0].x, vs = sc[0].y;
 #pragma unroll
             for (int i = 0; i + 2 < kStages; ++i) sc[i] = sc[i + 1];
-            sc[kStages - 2] = issue(it + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);
+            sc[kStages - 2] = issue(it + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
             cp_async_wait<kStages - 1>();
             __syncwarp();
             const int t0 = (span.lo + pa) * kPage + (warp + kWarps * it) * 32;
-            const unsigned char* st = ring + slot * kStage;
-            if (++slot == kStages) slot = 0;
+            const unsigned char* st = ring + stage * kStage;
+            if (++stage == kStages) stage = 0;
             if (!(t0 < keys_hi && t0 + 32 > keys_lo)) continue;
 
             // scores of 32 tokens: row g of group q (tile q / 2, its half q % 2) is token 8 (g / 2) + 2 q + g % 2
@@ -468,8 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
         }
         __syncthreads();
         const bool whole = pa == 0 && pb == np;
-        // blocks that share this (segment, head)
-        const int cf = whole ? blockIdx.x : owner(hb), cl = whole ? blockIdx.x : owner(hb + np - 1);
+        int cf, cl, slot;  // blocks that share this (segment, head), place of the first one's part
+        line.sharers(seg, h, hb, np, cf, cl, slot);
         constexpr int kPart = kMaxRows * 128 + 2 * kMaxRows;
         float* part = a.parts + (long long)(2 * blockIdx.x + (u != u0)) * kPart;
         constexpr int Q4 = D / 4;
@@ -520,8 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
             }
             __syncthreads();
             if (s_last) {
-                // a block's piece is its first one (slot 0) unless its share begins before this head
-                const float* p0 = a.parts + (long long)(2 * cf + (share(cf) < hb)) * kPart;
+                const float* p0 = a.parts + (long long)slot * kPart;
                 const float* p1 = a.parts + (long long)(2 * cf + 2) * kPart;  // of block cf + 1, then every second slot
                 for (int i = tid; i < span.rows * Q4; i += kThreads) {
                     const int r = i / Q4, q4 = i % Q4;

@@ -65,6 +65,75 @@ __device__ __forceinline__ RowScale row_scale(float top) {
     return {__uint_as_float((uint32_t)(267 - e) << 23), __uint_as_float((uint32_t)(e - 13) << 23)};
 }
 
+// How a launch's line of units (row block or tile, head, stretch of keys; heads
+// inside a segment) is cut into blocks: equal shares wherever they fall, or, where
+// that costs more, `parts` blocks for each (segment, head) -- short contexts, whose
+// pieces cost more to start and to join than the longest of them takes.
+struct Line {
+    const int* pref;  // units per head before each segment
+    int Hkv, q, r, parts, blocks;
+
+    // Costs in units: `least` units a block at least, `start` of a piece, `join` of joining pieces.
+    __device__ __forceinline__ Line(const int* prefix, int nseg, int nfull, int longest, int heads, int grid, int least, int start,
+                                    int join)
+        : pref(prefix), Hkv(heads), q(0), r(0), parts(0), blocks(0) {
+        const int U = prefix[nseg] * heads;  // below 2^31: the host bounds the launch
+        if (U == 0) return;
+        const int S = min(nfull, 1 << 20) * heads;
+        if (nfull == nseg && S <= grid) {
+            const int k = min(grid / S, (longest + least - 1) / least);
+            if ((longest + k - 1) / k + (k > 1 ? join : 0) <= (U + grid - 1) / grid + start + join) {
+                parts = k;
+                blocks = S * k;
+                return;
+            }
+        }
+        blocks = min(grid, max((U + least - 1) / least, S));
+        q = U / blocks;
+        r = U - q * blocks;  // the first r shares hold one unit more
+    }
+    __device__ __forceinline__ int share(int i) const { return q * i + min(i, r); }
+    __device__ __forceinline__ int owner(int x) const {
+        const int cut = r * (q + 1);
+        return x < cut ? x / (q + 1) : r + (x - cut) / q;
+    }
+    // Units [u0, u1) of a block, and the segment of the first.
+    __device__ __forceinline__ void range(int block, int nseg, int& u0, int& u1, int& seg) const {
+        if (parts) {
+            const int s = block / parts, part = block - s * parts;
+            seg = s / Hkv;
+            const int n = pref[seg + 1] - pref[seg], k = min(parts, n);
+            const int at = pref[seg] * Hkv + (s - seg * Hkv) * n;
+            u0 = part < k ? at + n * part / k : at;
+            u1 = part < k ? at + n * (part + 1) / k : at;
+            return;
+        }
+        u0 = share(block);
+        u1 = share(block + 1);
+        int lo = 0, hi = nseg - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (pref[mid] * Hkv <= u0) lo = mid;
+            else hi = mid - 1;
+        }
+        seg = lo;
+    }
+    // First and last block that share the n units from `at` on (head h of `seg`),
+    // and the slot of the first one's part: its first piece, unless its share
+    // begins before them.
+    __device__ __forceinline__ void sharers(int seg, int h, int at, int n, int& cf, int& cl, int& slot) const {
+        if (parts) {
+            cf = (seg * Hkv + h) * parts;
+            cl = cf + min(parts, n) - 1;
+            slot = 2 * cf;
+        } else {
+            cf = owner(at);
+            cl = owner(at + n - 1);
+            slot = 2 * cf + (share(cf) < at);
+        }
+    }
+};
+
 // Rows (tokens times heads of a group) per sequence from which attention goes
 // to attn_prefill.cu.  Measured, us for 16 / 24 / 32 rows, attn.cu's kernel (row
 // blocks of 16 and 32) against that one's: 24 sequences of 5,003 tokens, 4 kv
