@@ -494,7 +494,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
     } else if (warp >= kConvWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
         const int ct = tid - 32 * kConvWarp;
-        constexpr int KL = D / 32, CPR = D / 16;  // 16-byte loads per thread and tile of K (and of V); per K row
+        constexpr int KL = D / 32, KP = KL / 2;  // 16-byte loads per thread: of a tile of K (and of V), of a page
+        // This thread's 16 bytes of a page's first 4 KB of K (warps take four rows of
+        // 128 bytes, or eight of 64) and of V, and where their 32 bytes of fp16 go.
+        // Eight lanes that store together hold two rows and four neighbouring pieces,
+        // which the swizzle spreads over all banks.
+        const unsigned cw = (unsigned)ct >> 5, cl = (unsigned)ct & 31u;
+        const unsigned krow = D == 128 ? cw * 4 + (cl >> 4) * 2 + ((cl >> 2) & 1) : (unsigned)ct >> 2;
+        const unsigned katom = D == 128 ? (cl >> 3) & 1 : 0, kch = cl & 3, vrow = (unsigned)ct >> 2;
+        const unsigned kfrom = D == 128 ? krow * 8 + katom * 4 + kch : (unsigned)ct;
+        uint32_t kto[2], vto[2];
+#pragma unroll
+        for (unsigned e = 0; e < 2; ++e) {
+            kto[e] = base + SM::kK + katom * (kTileK * 128) + (krow >> 3) * 1024 + (krow & 7) * 128 + (((2 * kch + e) ^ (krow & 7)) << 4);
+            vto[e] = base + SM::kV + (vrow >> 3) * 1024 + (vrow & 7) * 128 + (((2 * kch + e) ^ (vrow & 7)) << 4);
+        }
         uint4 kr[KL], vr[KL];
         float sc[2] = {0.f, 0.f};
         // This thread's walk over the tiles of all pieces, one tile ahead of the conversion.
@@ -535,11 +549,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
         const uint4 none = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
         auto load_k = [&]() {
 #pragma unroll
-            for (int i = 0; i < KL; ++i) {
-                const int half = i / (KL / 2);  // a page is KL / 2 loads of 256 threads
-                kr[i] = nt.page[half] < 0 ? none
-                                          : __ldg(reinterpret_cast<const uint4*>(kbase + (long long)nt.page[half] * a.Hkv * (kPage * D)) +
-                                             (i % (KL / 2)) * 256 + ct);
+            for (int e = 0; e < 2; ++e) {
+                const uint4* src = reinterpret_cast<const uint4*>(kbase + (long long)max(nt.page[e], 0) * a.Hkv * (kPage * D)) + kfrom;
+#pragma unroll
+                for (int i = 0; i < KP; ++i) kr[e * KP + i] = nt.page[e] < 0 ? none : __ldg(src + i * 256);
             }
             if (ct < 2) {
                 const int p = ct == 0 ? nt.page[0] : nt.page[1];
@@ -550,25 +563,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
         };
         auto load_v = [&]() {
 #pragma unroll
-            for (int i = 0; i < KL; ++i) {
-                const int half = i / (KL / 2);
-                vr[i] = nt.page[half] < 0 ? none
-                                          : __ldg(reinterpret_cast<const uint4*>(vbase + (long long)nt.page[half] * a.Hkv * (kPage * D)) +
-                                             (i % (KL / 2)) * 256 + ct);
-            }
-        };
-        // sixteen codes as 32 bytes of fp16 at chunks c, c + 1 of row r: K's as c * 2^-24,
-        // V's as signed integers (`swap`: the second chunk first)
-        auto store = [&](uint32_t atom, int r, int c, bool swap, bool raw, const uint4& v) {
-            const uint32_t row = atom + (r >> 3) * 1024 + (r & 7) * 128;
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int q = swap ? 1 - e : e;
-                const uint32_t x = q ? w[2] : w[0], y = q ? w[3] : w[1];
-                const uint32_t to = row + (((c + q) ^ (r & 7)) << 4);
-                if (raw) sts16(to, codes_raw(x, 0x4140), codes_raw(x, 0x4342), codes_raw(y, 0x4140), codes_raw(y, 0x4342));
-                else sts16(to, codes_f16x2(x, 0x4140), codes_f16x2(x, 0x4342), codes_f16x2(y, 0x4140), codes_f16x2(y, 0x4342));
+                const uint4* src = reinterpret_cast<const uint4*>(vbase + (long long)max(nt.page[e], 0) * a.Hkv * (kPage * D)) + ct;
+#pragma unroll
+                for (int i = 0; i < KP; ++i) vr[e * KP + i] = nt.page[e] < 0 ? none : __ldg(src + i * 256);
             }
         };
         bool ok = true, more = advance();
@@ -585,12 +583,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
                 o[1] = sc[1] == 0.f ? 0.f : __log2f(sc[1]);  // a page of zeros keeps its weight in the sum
                 o[2] = sc[1] == 0.f ? 1.f : __fdividef(1.f, sc[1]);
             }
-            const uint32_t kt = base + SM::kK + st * SM::kKTile;
+            // K as c * 2^-24; the second page's rows follow the first's 64, 4 KB of codes are 32 or 64 rows
 #pragma unroll
             for (int i = 0; i < KL; ++i) {
-                const int ci = (i % (KL / 2)) * 256 + ct, r = ci / CPR + (i / (KL / 2)) * kPage, ch = ci % CPR;
-                // 64 elements an atom; lanes of the second atom store their halves the other way round (banks)
-                store(kt + (ch >> 2) * (kTileK * 128), r, (ch & 3) * 2, D == 128 && (ch & 4), true, kr[i]);
+                const uint32_t at = st * SM::kKTile + (i / KP) * (kPage * 128) + (i % KP) * (32 * 128);
+                sts16(kto[0] + at, codes_raw(kr[i].x, 0x4140), codes_raw(kr[i].x, 0x4342), codes_raw(kr[i].y, 0x4140), codes_raw(kr[i].y, 0x4342));
+                sts16(kto[1] + at, codes_raw(kr[i].z, 0x4140), codes_raw(kr[i].z, 0x4342), codes_raw(kr[i].w, 0x4140), codes_raw(kr[i].w, 0x4342));
             }
             fence_async();
             mbar_arrive(&b_kfull[st]);
@@ -598,11 +596,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             if (more) load_k();
             if (j >= 2) ok = wait(&b_vempty[st], ph);
             if (!ok) break;
-            const uint32_t vt = base + SM::kV + st * SM::kVTile;
+            // V as signed integers; each page is an atom of its own, 4 KB of codes are 64 dimensions
 #pragma unroll
             for (int i = 0; i < KL; ++i) {
-                const int ci = (i % (KL / 2)) * 256 + ct;  // row d = ci / 4, 16 tokens of the page
-                store(vt + (i / (KL / 2)) * (D * 128), ci >> 2, (ci & 3) * 2, false, false, vr[i]);
+                const uint32_t at = st * SM::kVTile + (i / KP) * (D * 128) + (i % KP) * (64 * 128);
+                sts16(vto[0] + at, codes_f16x2(vr[i].x, 0x4140), codes_f16x2(vr[i].x, 0x4342), codes_f16x2(vr[i].y, 0x4140),
+                      codes_f16x2(vr[i].y, 0x4342));
+                sts16(vto[1] + at, codes_f16x2(vr[i].z, 0x4140), codes_f16x2(vr[i].z, 0x4342), codes_f16x2(vr[i].w, 0x4140),
+                      codes_f16x2(vr[i].w, 0x4342));
             }
             fence_async();
             mbar_arrive(&b_vfull[st]);
