@@ -322,7 +322,7 @@ int momij_attention(const void* q, long long ldq, void* out, long long ldo, cons
 
 /* y[m, n] = sum_k (s[n, k/gs] * q[n, k] + b[n, k/gs]) * x[m, k] with 4-bit codes
  * (MLX affine, transpose=true): w uint32 [N, K/8], code k at bits [4(k%8),
- * 4(k%8)+3]; s, b 16-bit [N, K/gs], gs 64 or 128, K % gs == 0; w 8-byte aligned.
+ * 4(k%8)+3]; s, b 16-bit [N, K/gs], gs 64 or 128, K % gs == 0; w 16-byte aligned.
  * Rows of x and y are ldx and ldy elements apart.  For few tokens: up to 32 share
  * a pass over the matrix (fewer for K above 3,000 or so).
  * Replaces: the 4-bit output head's product (SeedlessMetal.swift:2598-2716) and

@@ -16,10 +16,13 @@
 //     nothing is rounded but elements below 2^-38 of the token's largest.
 //   * s, b, the group sums and the running sums are fp32; y is rounded once.
 //
-// What bounds it: the bytes of the matrix (K/2 + 4 K/gs per row).  A batch of
-// 256 columns of 16 rows is 2 KB of codes per warp, loaded straight into
-// registers (a lane's 8 bytes are the 16 codes it multiplies), the next batch
-// while this one is multiplied.
+// What bounds it: the bytes of the matrix (K/2 + 4 K/gs per row), as long as the
+// instructions per code stay below what the bytes' arrival allows (46 codes per
+// cycle and SM at the copy rate).  A batch is 256 columns of 16 rows: 2 KB of
+// codes and the scales and biases, which a warp copies asynchronously into a ring
+// of its own in shared memory, three batches ahead.  (With the batch after the
+// present one in registers instead: 50 us for 151,936 x 2,048 and one token; the
+// registers left room for 24 warps with 3 KB each in flight.)
 #include <algorithm>
 
 #include "host.cuh"
@@ -27,10 +30,12 @@
 namespace momij {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMaxWarps = 16;
 constexpr int kBlk = 64;         // columns per block: a warp row's 32 bytes of codes
 constexpr int kBatchBlks = 4;    // blocks per batch
 constexpr int kMaxTok = 32;      // tokens per pass (four column tiles)
+constexpr int kStages = 4;       // of a warp's ring
+constexpr int kStageCodes = 16 * kBatchBlks * 32, kStage = kStageCodes + 2 * 16 * 8;  // codes, scales, biases
 
 struct Args {
     const uint16_t* x;
@@ -43,7 +48,7 @@ struct Args {
     int M, N, K, mt;             // mt: tokens per pass (blockIdx.y)
     int wk;                      // warps that share a row tile, each with every wk-th batch
     int xvec;                    // x rows are 16-byte aligned
-    int off_xs, off_red, off_e;  // dynamic shared memory: x operand at 0
+    int off_x, off_xs, off_red, off_e;  // dynamic shared memory; the rings at 0
     int pitch;                   // bytes per token of the x operand
 };
 
@@ -54,93 +59,86 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint2 ldg8(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
 __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
 
-// One batch of one row tile: the lane's codes of rows g and g + 8, and the
-// batch's scales and biases of both rows (groups per batch: 4 or 2).
-template <int GPB>
-struct Batch {
-    uint2 w[kBatchBlks][2];
-    uint32_t s[2][GPB / 2], b[2][GPB / 2];
-};
-
-template <int GPB, bool VEC>
-__device__ __forceinline__ void load_groups(uint32_t (&v)[GPB / 2], const uint16_t* row, int g0, int ng) {
-    if (VEC) {
-        if (GPB == 4) {
-            const uint2 t = g0 < ng ? ldg8(row + g0) : make_uint2(0u, 0u);
-            v[0] = t.x;
-            v[GPB / 2 - 1] = t.y;
-        } else {
-            v[0] = g0 < ng ? __ldg(reinterpret_cast<const uint32_t*>(row + g0)) : 0u;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < GPB / 2; ++i) {
-            const uint32_t lo = g0 + 2 * i < ng ? __ldg(row + g0 + 2 * i) : 0;
-            const uint32_t hi = g0 + 2 * i + 1 < ng ? __ldg(row + g0 + 2 * i + 1) : 0;
-            v[i] = lo | (hi << 16);
-        }
-    }
+// The two 16-bit values of a word as floats.
+template <int DT>
+__device__ __forceinline__ float half_of(uint32_t w, int hi) {
+    if (DT == MOMIJ_DTYPE_BF16) return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
+    return Half<DT>::to_f((uint16_t)(hi ? w >> 16 : w & 0xffffu));
 }
 
-template <int DT, int NT, int GS, bool VEC>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) qmm4_kernel(const Args a) {
+// ONE: a pass of a single token, which is column 0.  VEC: a batch's scales of a
+// row are one aligned copy; otherwise they are read where they are used.
+template <int DT, int NT, int GS, bool VEC, bool ONE>
+__global__ void __launch_bounds__(kMaxWarps * 32, 1) qmm4_kernel(const Args a) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int GPB = kBatchBlks * kBlk / GS;
+    constexpr int GPB = kBatchBlks * kBlk / GS;               // groups per batch: 4 or 2
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+    const int threads = blockDim.x, warps = threads >> 5;
+    unsigned char* sx = smem + a.off_x;                       // x operand, `pitch` bytes per token
     float* xs = reinterpret_cast<float*>(smem + a.off_xs);    // [group][8 NT]: sums of x, scaled like the products
     float* red = reinterpret_cast<float*>(smem + a.off_red);  // [2][warp][8 NT][17]
     unsigned* s_e = reinterpret_cast<unsigned*>(smem + a.off_e);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     const int m0 = blockIdx.y * a.mt, mt = min(a.mt, a.M - m0);
     const int ng = a.K / GS, nblk = a.K / kBlk, nbatch = (nblk + kBatchBlks - 1) / kBatchBlks;
-    const int wk = a.wk, wr = kWarps / wk, kw = warp % wk, rw = warp / wk;
+    const int wk = a.wk, wr = warps / wk, kw = warp % wk, rw = warp / wk;
     const int ntiles = (a.N + 15) / 16, nround = (ntiles + wr - 1) / wr;
 
     if (tid < kMaxTok) s_e[tid] = 0;
     pdl_wait();
     if (__syncthreads_or(tid == 0 && a.stop && __ldcg(a.stop) != 0)) return;
 
-    Batch<GPB> bat[2];
-    // flattened walk over (round, batch); the load runs one item ahead
-    int lr = blockIdx.x, lk = kw;
-    auto load = [&](Batch<GPB>& f) {
-        if (lr < nround) {
-            const int r0 = min((lr * wr + rw) * 16 + g, a.N - 1), r1 = min((lr * wr + rw) * 16 + g + 8, a.N - 1);
-            const long long wrow = a.K / 8;  // words per row
-            const uint32_t* w0 = a.w + r0 * wrow + lk * (kBatchBlks * 8) + 2 * c;
-            const uint32_t* w1 = a.w + r1 * wrow + lk * (kBatchBlks * 8) + 2 * c;
+    // ---- the ring: a flattened walk over (round, batch), three items ahead --------
+    // A lane copies 16 bytes of rows lane / 8 + 4 i; a row's four 32-byte blocks are
+    // rotated by the row, so that the reads of four rows cover all banks.
+    const uint32_t ring = smem_u32(smem) + warp * (kStages * kStage);
+    const int crow = lane >> 3, cch = lane & 7;
+    const uint32_t cdst = crow * 128 + ((((cch >> 1) ^ crow) & 3) << 5) + ((cch & 1) << 4);  // (rows + 4 i keep the rotation)
+    int lr = blockIdx.x, lk = kw, lst = 0;
+    const unsigned char* wp[4] = {};
+    const uint16_t* gp = nullptr;
+    auto rows = [&]() {  // this round's rows; past the end the last one again, unwritten
+        const int row0 = (lr * wr + rw) * 16;
 #pragma unroll
-            for (int i = 0; i < kBatchBlks; ++i) {
-                const bool in = lk * kBatchBlks + i < nblk;
-                f.w[i][0] = in ? ldg8(w0 + 8 * i) : make_uint2(0u, 0u);
-                f.w[i][1] = in ? ldg8(w1 + 8 * i) : make_uint2(0u, 0u);
-            }
-            load_groups<GPB, VEC>(f.s[0], a.s + (long long)r0 * ng, lk * GPB, ng);
-            load_groups<GPB, VEC>(f.s[1], a.s + (long long)r1 * ng, lk * GPB, ng);
-            load_groups<GPB, VEC>(f.b[0], a.b + (long long)r0 * ng, lk * GPB, ng);
-            load_groups<GPB, VEC>(f.b[1], a.b + (long long)r1 * ng, lk * GPB, ng);
-        }
-        lk += wk;
-        if (lk >= nbatch) {
-            lk = kw;
-            lr += gridDim.x;
-        }
+        for (int i = 0; i < 4; ++i)
+            wp[i] = reinterpret_cast<const unsigned char*>(a.w) + (long long)min(row0 + crow + 4 * i, a.N - 1) * (a.K / 2) + cch * 16;
+        // lanes 0-15 the scales of row `lane`, 16-31 the biases
+        gp = (lane < 16 ? a.s : a.b) + (long long)min(row0 + (lane & 15), a.N - 1) * ng;
     };
-    load(bat[0]);
+    if (lr < nround) rows();
+    auto issue = [&]() {
+        if (lr < nround) {
+            const uint32_t dst = ring + lst * kStage;
+            const bool in = lk * kBatchBlks + (cch >> 1) < nblk;  // past the row's end: zeros
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cp_async16(dst + cdst + i * 512, in ? wp[i] + lk * (kBatchBlks * 32) : wp[i], in);
+            if (VEC) {
+                const uint32_t gd = dst + kStageCodes + lane * 8;
+                if (GPB == 4) cp_async8(gd, gp + lk * GPB, true);
+                else cp_async4(gd, gp + lk * GPB, true);
+            }
+            if (++lst == kStages) lst = 0;
+            lk += wk;
+            if (lk >= nbatch) {
+                lk = kw;
+                lr += gridDim.x;
+                if (lr < nround) rows();
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue();
 
     // ---- x: largest magnitude per token (as bits, so that NaN counts as the
-    // largest), then the permuted fp16 operand and the group sums -------------
-    const int nc = a.K / 8;  // 8-element pieces per token
+    // largest), then the permuted fp16 operand and the group sums; the pieces of
+    // all tokens in one line ----------------------------------------------------
+    const int nc = a.K / 8, np = mt * nc;  // 8-element pieces per token, in all
     auto piece = [&](int m, int p) -> uint4 {
         const uint16_t* src = a.x + (m0 + m) * a.ldx + 8 * p;
         if (a.xvec) return __ldg(reinterpret_cast<const uint4*>(src));
@@ -149,44 +147,65 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) qmm4_kernel(const A
         for (int i = 0; i < 4; ++i) v[i] = __ldg(src + 2 * i) | ((uint32_t)__ldg(src + 2 * i + 1) << 16);
         return make_uint4(v[0], v[1], v[2], v[3]);
     };
-    for (int m = 0; m < mt; ++m) {
-        uint32_t top = 0;
-        for (int p = tid; p < nc; p += kThreads) {
-            const uint4 v = piece(m, p);
-            const uint32_t t[4] = {v.x, v.y, v.z, v.w};
+    for (int i0 = 0; i0 < np; i0 += 2 * threads) {
+        uint4 v[2];
+        int m[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int i = i0 + k * threads + tid;
+            m[k] = ONE ? 0 : min(i / nc, mt - 1);
+            v[k] = make_uint4(0u, 0u, 0u, 0u);
+            if (i < np) v[k] = piece(m[k], i - m[k] * nc);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (i0 + k * threads + (warp << 5) >= np) break;
+            const uint32_t t[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+            uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = max(top, max(t[i] & 0x7fffu, (t[i] >> 16) & 0x7fffu));
+            const int first = __shfl_sync(0xffffffffu, m[k], 0);  // most warps hold one token's pieces
+            if (ONE || __all_sync(0xffffffffu, m[k] == first)) {
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0 && top) atomicMax(s_e + first, top);
+            } else if (top) {
+                atomicMax(s_e + m[k], top);
+            }
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) atomicMax(s_e + m, top);
     }
     __syncthreads();
-    // exponent shift of a token: its largest magnitude becomes 2^14 .. 2^15
-    // (0 for a token of zeros, or one with infinities or NaN)
-    auto shift_of = [&](int m) -> int {
-        const float f = Half<DT>::to_f((uint16_t)s_e[m]);
-        const uint32_t u = __float_as_uint(f);
-        if (u == 0 || u >= 0x7f800000u) return 0;
-        return 14 - ilogbf(f);
+    // A token's biased exponent, from which x is scaled so that its largest
+    // magnitude becomes 2^14 .. 2^15; 141 (a factor of one) for zeros, infinities and
+    // NaN.  Tokens below 2^-112 stay smaller.
+    auto exponent = [&](int m) -> int {
+        const uint32_t u = __float_as_uint(Half<DT>::to_f((uint16_t)s_e[m]));
+        return u == 0 || u >= 0x7f800000u ? 141 : max((int)(u >> 23), 15);
     };
-    for (int m = 0; m < mt; ++m) {
-        const int sh = shift_of(m);
-        // two steps: 2^sh alone can leave fp32's range
-        const float f0 = ldexpf(1.f, sh / 2), f1 = ldexpf(1.f, sh - sh / 2);
-        for (int p0 = 0; p0 < nc; p0 += kThreads) {
-            const int p = p0 + tid;
-            float sum = 0.f;
-            if (p < nc) {
-                const uint4 v = piece(m, p);
-                const uint32_t t[4] = {v.x, v.y, v.z, v.w};
-                float e[8];
+    for (int i0 = 0; i0 < np; i0 += 2 * threads) {
+        uint4 v[2];
+        int m[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    e[2 * i] = Half<DT>::to_f((uint16_t)(t[i] & 0xffffu)) * f0 * f1;
-                    e[2 * i + 1] = Half<DT>::to_f((uint16_t)(t[i] >> 16)) * f0 * f1;
-                }
+        for (int k = 0; k < 2; ++k) {
+            const int i = i0 + k * threads + tid;
+            m[k] = ONE ? 0 : min(i / nc, mt - 1);
+            v[k] = make_uint4(0u, 0u, 0u, 0u);
+            if (i < np) v[k] = piece(m[k], i - m[k] * nc);
+        }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += e[i];
+        for (int k = 0; k < 2; ++k) {
+            const int i = i0 + k * threads + tid, p = i - m[k] * nc;
+            if (i0 + k * threads + (warp << 5) >= np) break;
+            const float f = __uint_as_float((uint32_t)(268 - exponent(m[k])) << 23);
+            const uint32_t t[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+            float e[8], sum = 0.f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                e[2 * q] = half_of<DT>(t[q], 0) * f;
+                e[2 * q + 1] = half_of<DT>(t[q], 1) * f;
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) sum += e[q];
+            if (i < np) {
                 uint4 o;
                 o.x = f16x2(e[0], e[4]);
                 o.y = f16x2(e[1] * 0.0625f, e[5] * 0.0625f);
@@ -194,25 +213,53 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) qmm4_kernel(const A
                 o.w = f16x2(e[3] * 0.0625f, e[7] * 0.0625f);
                 // piece p = (block, lane c, word j): the lane's pieces of one word lie side by side
                 const int blk = p >> 3, pc = (p >> 1) & 3, j = p & 1;
-                *reinterpret_cast<uint4*>(smem + m * a.pitch + blk * 128 + j * 64 + pc * 16) = o;
+                *reinterpret_cast<uint4*>(sx + m[k] * a.pitch + blk * 128 + j * 64 + pc * 16) = o;
             }
 #pragma unroll
             for (int o = 1; o < GS / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             // 2^-24: the unit of the codes' products
-            if (p < nc && (p & (GS / 8 - 1)) == 0) xs[(p / (GS / 8)) * (8 * NT) + m] = sum * 5.9604644775390625e-08f;
+            if (i < np && (p & (GS / 8 - 1)) == 0) xs[(p / (GS / 8)) * (8 * NT) + m[k]] = sum * 5.9604644775390625e-08f;
         }
     }
     __syncthreads();
 
     const unsigned char* xrow[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) xrow[n] = smem + min(8 * n + g, mt - 1) * a.pitch + c * 16;
+    for (int n = 0; n < NT; ++n) xrow[n] = sx + (ONE ? 0 : min(8 * n + g, mt - 1) * a.pitch) + c * 16;
+    const unsigned char* mine = smem + warp * (kStages * kStage);
+    const unsigned char* crow0 = mine + g * 128 + c * 8;  // rows g and g + 8 of a stage; block i at i ^ (g & 3)
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    int round = blockIdx.x, kb = kw, buf = 0;
-
-    auto step = [&](const Batch<GPB>& f) {
+    int kb = kw, buf = 0, st = 0;
+    for (int round = blockIdx.x; round < nround;) {
+        issue();
+        cp_async_wait<kStages - 1>();
+        __syncwarp();
+        const unsigned char* wc = crow0 + st * kStage;
+        const unsigned char* sc = mine + st * kStage + kStageCodes + g * 8;
+        const int row0 = (round * wr + rw) * 16;
+        uint32_t sg[2][2][GPB / 2];  // [scale, bias][row][pair of groups]
+        if (VEC) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t* o = sg[e >> 1][e & 1];
+                const unsigned char* p = sc + (e >> 1) * 128 + (e & 1) * 64;
+                if (GPB == 4) *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(p);
+                else o[0] = *reinterpret_cast<const uint32_t*>(p);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint16_t* p = (e >> 1 ? a.b : a.s) + (long long)min(row0 + g + 8 * (e & 1), a.N - 1) * ng;
+#pragma unroll
+                for (int i = 0; i < GPB / 2; ++i) {
+                    const int q = kb * GPB + 2 * i;
+                    sg[e >> 1][e & 1][i] = (q < ng ? __ldg(p + q) : 0) | ((uint32_t)(q + 1 < ng ? __ldg(p + q + 1) : 0) << 16);
+                }
+            }
+        }
+        const bool full = (kb + 1) * kBatchBlks <= nblk;  // else: zero codes, scales and biases against whatever is last
 #pragma unroll
         for (int gi = 0; gi < GPB; ++gi) {
             float d[NT][4];
@@ -221,10 +268,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) qmm4_kernel(const A
 #pragma unroll
             for (int bi = 0; bi < GS / kBlk; ++bi) {
                 const int i = gi * (GS / kBlk) + bi;
-                const int blk = min(kb * kBatchBlks + i, nblk - 1);  // past the end: zero codes, scales and biases
+                const int blk = full ? kb * kBatchBlks + i : min(kb * kBatchBlks + i, nblk - 1);
+                const uint2 c0 = *reinterpret_cast<const uint2*>(wc + ((i ^ (g & 3)) << 5));
+                const uint2 c1 = *reinterpret_cast<const uint2*>(wc + 1024 + ((i ^ (g & 3)) << 5));
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const uint32_t u0 = j ? f.w[i][0].y : f.w[i][0].x, u1 = j ? f.w[i][1].y : f.w[i][1].x;
+                    const uint32_t u0 = j ? c0.y : c0.x, u1 = j ? c1.y : c1.x;
                     const uint32_t h0 = u0 >> 8, h1 = u1 >> 8;
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
@@ -234,65 +283,75 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) qmm4_kernel(const A
                     }
                 }
             }
-            const int grp = min(kb * GPB + gi, ng - 1);
-            const uint32_t sw0 = f.s[0][gi / 2], sw1 = f.s[1][gi / 2], bw0 = f.b[0][gi / 2], bw1 = f.b[1][gi / 2];
-            const float s0 = Half<DT>::to_f((uint16_t)(gi & 1 ? sw0 >> 16 : sw0 & 0xffffu));
-            const float s1 = Half<DT>::to_f((uint16_t)(gi & 1 ? sw1 >> 16 : sw1 & 0xffffu));
-            const float b0 = Half<DT>::to_f((uint16_t)(gi & 1 ? bw0 >> 16 : bw0 & 0xffffu));
-            const float b1 = Half<DT>::to_f((uint16_t)(gi & 1 ? bw1 >> 16 : bw1 & 0xffffu));
+            const int grp = full ? kb * GPB + gi : min(kb * GPB + gi, ng - 1);
+            const float sc0 = half_of<DT>(sg[0][0][gi / 2], gi & 1), sc1 = half_of<DT>(sg[0][1][gi / 2], gi & 1);
+            const float bi0 = half_of<DT>(sg[1][0][gi / 2], gi & 1), bi1 = half_of<DT>(sg[1][1][gi / 2], gi & 1);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float2 t = *reinterpret_cast<const float2*>(xs + grp * (8 * NT) + 8 * n + 2 * c);
-                acc[n][0] = fmaf(b0, t.x, fmaf(s0, d[n][0], acc[n][0]));
-                acc[n][1] = fmaf(b0, t.y, fmaf(s0, d[n][1], acc[n][1]));
-                acc[n][2] = fmaf(b1, t.x, fmaf(s1, d[n][2], acc[n][2]));
-                acc[n][3] = fmaf(b1, t.y, fmaf(s1, d[n][3], acc[n][3]));
+                const float* t = xs + grp * (8 * NT) + (ONE ? 0 : 8 * n + 2 * c);
+                const float t0 = t[0];
+                acc[n][0] = fmaf(bi0, t0, fmaf(sc0, d[n][0], acc[n][0]));
+                acc[n][2] = fmaf(bi1, t0, fmaf(sc1, d[n][2], acc[n][2]));
+                if (!ONE) {
+                    const float t1 = t[1];
+                    acc[n][1] = fmaf(bi0, t1, fmaf(sc0, d[n][1], acc[n][1]));
+                    acc[n][3] = fmaf(bi1, t1, fmaf(sc1, d[n][3], acc[n][3]));
+                }
             }
         }
+        __syncwarp();  // the stage is free for the copies issued next
+        if (++st == kStages) st = 0;
         kb += wk;
-        if (kb < nbatch) return;
-        // the round's last batch of this warp: sum the wk warps of each tile
-        float* mine = red + (buf * kWarps + warp) * (8 * NT * 17);
+        if (kb < nbatch) continue;
+        // the round's last batch of this warp: sum the wk warps of the tile, in order
+        float* part = red + (buf * warps + warp) * (8 * NT * 17);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            mine[(8 * n + 2 * c) * 17 + g] = acc[n][0];
-            mine[(8 * n + 2 * c + 1) * 17 + g] = acc[n][1];
-            mine[(8 * n + 2 * c) * 17 + g + 8] = acc[n][2];
-            mine[(8 * n + 2 * c + 1) * 17 + g + 8] = acc[n][3];
+            if (!ONE || c == 0) {
+                part[(8 * n + 2 * c) * 17 + g] = acc[n][0];
+                part[(8 * n + 2 * c) * 17 + g + 8] = acc[n][2];
+            }
+            if (!ONE) {
+                part[(8 * n + 2 * c + 1) * 17 + g] = acc[n][1];
+                part[(8 * n + 2 * c + 1) * 17 + g + 8] = acc[n][3];
+            }
             acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
         }
-        __syncthreads();
-        for (int o = tid; o < mt * wr * 16; o += kThreads) {
-            const int m = o / (wr * 16), rr = o - m * (wr * 16), t = rr >> 4, row = round * wr * 16 + rr;
-            const float* p = red + (buf * kWarps + t * wk) * (8 * NT * 17) + m * 17 + (rr & 15);
+        if (wk == 1) __syncwarp();
+        else if (wk == warps) __syncthreads();
+        else bar_sync(1 + rw, 32 * wk);
+        const float* first = red + (buf * warps + rw * wk) * (8 * NT * 17);
+        for (int o = kw * 32 + lane; o < mt * 16; o += 32 * wk) {
+            const int m = o >> 4, r = o & 15;
             float v = 0.f;
-            for (int k = 0; k < wk; ++k) v += p[k * (8 * NT * 17)];
-            if (row < a.N) a.y[(m0 + m) * a.ldy + row] = Half<DT>::from_f(ldexpf(v, 24 - shift_of(m)));
+            for (int k = 0; k < wk; ++k) v += first[k * (8 * NT * 17) + m * 17 + r];
+            if (row0 + r < a.N) a.y[(m0 + m) * a.ldy + row0 + r] = Half<DT>::from_f(ldexpf(v, exponent(m) - 117));
         }
         buf ^= 1;  // the next round writes the other half: one barrier a round
         kb = kw;
         round += gridDim.x;
-    };
-    while (round < nround) {
-        load(bat[1]);
-        step(bat[0]);
-        if (round >= nround) break;
-        load(bat[0]);
-        step(bat[1]);
     }
+    cp_async_wait<0>();
     pdl_launch_dependents();
 }
 
-template <int DT, int NT, int GS, bool VEC>
-int launch(const Args& a, dim3 grid, size_t smem, momij_stream_t st) {
+template <int DT, int NT, int GS, bool VEC, bool ONE>
+int launch(const Args& a, dim3 grid, int warps, size_t smem, momij_stream_t st) {
     static int granted[64];
-    if (!host_allow_smem(qmm4_kernel<DT, NT, GS, VEC>, smem, granted)) return MOMIJ_ERR_CUDA;
-    return host_launch(qmm4_kernel<DT, NT, GS, VEC>, grid, dim3(kThreads), smem, st, a);
+    if (!host_allow_smem(qmm4_kernel<DT, NT, GS, VEC, ONE>, smem, granted)) return MOMIJ_ERR_CUDA;
+    return host_launch(qmm4_kernel<DT, NT, GS, VEC, ONE>, grid, dim3(32 * warps), smem, st, a);
 }
-template <int DT, int NT>
-int launch_nt(const Args& a, dim3 grid, size_t smem, int gs, bool vec, momij_stream_t st) {
-    if (gs == 64) return vec ? launch<DT, NT, 64, true>(a, grid, smem, st) : launch<DT, NT, 64, false>(a, grid, smem, st);
-    return vec ? launch<DT, NT, 128, true>(a, grid, smem, st) : launch<DT, NT, 128, false>(a, grid, smem, st);
+template <int DT, int NT, bool ONE>
+int launch_nt(const Args& a, dim3 grid, int warps, size_t smem, int gs, bool vec, momij_stream_t st) {
+    if (gs == 64) return vec ? launch<DT, NT, 64, true, ONE>(a, grid, warps, smem, st) : launch<DT, NT, 64, false, ONE>(a, grid, warps, smem, st);
+    return vec ? launch<DT, NT, 128, true, ONE>(a, grid, warps, smem, st) : launch<DT, NT, 128, false, ONE>(a, grid, warps, smem, st);
+}
+template <int DT>
+int launch_dt(const Args& a, dim3 grid, int warps, size_t smem, int nt, int gs, bool vec, momij_stream_t st) {
+    if (a.mt == 1) return launch_nt<DT, 1, true>(a, grid, warps, smem, gs, vec, st);
+    if (nt == 1) return launch_nt<DT, 1, false>(a, grid, warps, smem, gs, vec, st);
+    if (nt == 2) return launch_nt<DT, 2, false>(a, grid, warps, smem, gs, vec, st);
+    return launch_nt<DT, 4, false>(a, grid, warps, smem, gs, vec, st);
 }
 
 }  // namespace
@@ -308,7 +367,7 @@ extern "C" int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const
     if ((gs != 64 && gs != 128) || K < gs || K % gs != 0) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     if (M == 0 || N == 0) return MOMIJ_OK;
     if (!x || !w || !scales || !biases || !y || ldx < K || ldy < N) return MOMIJ_ERR_INVALID_ARGUMENT;
-    if (!host_aligned(w, 8) || !host_aligned(scales, 2) || !host_aligned(biases, 2) || !host_aligned(x, 2) || !host_aligned(y, 2))
+    if (!host_aligned(w, 16) || !host_aligned(scales, 2) || !host_aligned(biases, 2) || !host_aligned(x, 2) || !host_aligned(y, 2))
         return MOMIJ_ERR_INVALID_ARGUMENT;
     const int sms = host_sm_count();
     if (sms <= 0) return MOMIJ_ERR_CUDA;
@@ -329,42 +388,44 @@ extern "C" int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const
     const int ng = K / gs;
     const bool vec = gs == 64 ? ng % 4 == 0 && host_aligned(scales, 8) && host_aligned(biases, 8)
                               : ng % 2 == 0 && host_aligned(scales, 4) && host_aligned(biases, 4);
-    // tokens per pass: up to 32, fewer where their operand would not fit
     a.pitch = 2 * K + 64;  // 64 bytes more: the tokens of a read start on different banks
-    constexpr size_t kBudget = 200 * 1024;
-    auto bytes = [&](int mt) {
-        const int cols = 8 * (mt <= 8 ? 1 : mt <= 16 ? 2 : 4);
-        return (size_t)mt * a.pitch + (size_t)ng * cols * 4 + (size_t)2 * kWarps * cols * 17 * 4 + 4 * kMaxTok;
+    const int ntiles = (N + 15) / 16, nbatch = (K / kBlk + kBatchBlks - 1) / kBatchBlks;
+    auto cols = [](int mt) { return 8 * (mt <= 8 ? 1 : mt <= 16 ? 2 : 4); };
+    auto bytes = [&](int mt, int warps) {
+        return (size_t)warps * kStages * kStage + (size_t)mt * a.pitch + (size_t)ng * cols(mt) * 4 +
+               (size_t)2 * warps * cols(mt) * 17 * 4 + 4 * kMaxTok;
     };
+    constexpr size_t kBudget = 224 * 1024;
+    // Warps per block (one block an SM) and warps that share a row tile.  Sixteen
+    // warps keep the copies going where their rings leave room for the tokens;
+    // eight where they do not, or where sixteen would leave SMs without a round.
+    // A tile is shared by the fewest warps (1, 2, 4, 8, at most one a batch) that
+    // leave every warp eight items or more, so that the last, partly filled round
+    // costs little; small matrices end at eight, which spreads their rows over the SMs.
+    int warps = kMaxWarps;
+    auto share = [&](int w) {
+        int k = 1;
+        while (k < 8 && 2 * k <= nbatch && (long long)ntiles * k < 8LL * sms * w) k *= 2;
+        return k;
+    };
+    if ((long long)ntiles * share(16) <= 16LL * sms / 2 || bytes(std::min(M, 8), 16) > kBudget) warps = 8;
+    // tokens per pass: up to 32, fewer where their operand would not fit
     int mt = std::min(M, kMaxTok);
-    while (mt > 1 && bytes(mt) > kBudget) --mt;
-    if (bytes(mt) > kBudget) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
+    while (mt > 1 && bytes(mt, warps) > kBudget) --mt;
+    if (bytes(mt, warps) > kBudget) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     const int passes = (M + mt - 1) / mt;
     mt = (M + passes - 1) / passes;
     a.mt = mt;
-    const int nt = mt <= 8 ? 1 : mt <= 16 ? 2 : 4;
-    a.off_xs = mt * a.pitch;
+    const int nt = cols(mt) / 8;
+    a.off_x = warps * kStages * kStage;
+    a.off_xs = a.off_x + mt * a.pitch;
     a.off_red = a.off_xs + ng * 8 * nt * 4;
-    a.off_e = a.off_red + 2 * kWarps * 8 * nt * 17 * 4;
-    const size_t smem = bytes(mt);
-    const int resident = std::max(1, std::min(nt == 1 ? 3 : 2, (int)(220 * 1024 / (smem + 1024))));
-    // Warps that share a row tile: the fewest (1, 2, 4, 8, at most one a
-    // batch) that leave every warp slot eight items or more, so that the last,
-    // partly filled round costs little; small matrices end at eight, which
-    // also spreads their few rows over the SMs.
-    const int ntiles = (N + 15) / 16, nbatch = (K / kBlk + kBatchBlks - 1) / kBatchBlks;
-    int wk = 1;
-    while (wk < kWarps && 2 * wk <= nbatch && (long long)ntiles * wk < 8LL * sms * resident * kWarps) wk *= 2;
-    a.wk = wk;
-    const int wr = kWarps / wk, nround = (ntiles + wr - 1) / wr;
+    a.off_e = a.off_red + 2 * warps * 8 * nt * 17 * 4;
+    const size_t smem = bytes(mt, warps);
+    a.wk = share(warps);
+    const int wr = warps / a.wk, nround = (ntiles + wr - 1) / wr;
     if (passes > 65535) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
-    const dim3 grid(std::min(nround, sms * resident), passes);
-    if (dtype == MOMIJ_DTYPE_BF16) {
-        if (nt == 1) return launch_nt<MOMIJ_DTYPE_BF16, 1>(a, grid, smem, gs, vec, stream);
-        if (nt == 2) return launch_nt<MOMIJ_DTYPE_BF16, 2>(a, grid, smem, gs, vec, stream);
-        return launch_nt<MOMIJ_DTYPE_BF16, 4>(a, grid, smem, gs, vec, stream);
-    }
-    if (nt == 1) return launch_nt<MOMIJ_DTYPE_F16, 1>(a, grid, smem, gs, vec, stream);
-    if (nt == 2) return launch_nt<MOMIJ_DTYPE_F16, 2>(a, grid, smem, gs, vec, stream);
-    return launch_nt<MOMIJ_DTYPE_F16, 4>(a, grid, smem, gs, vec, stream);
+    const dim3 grid(std::min(nround, sms), passes);
+    return dtype == MOMIJ_DTYPE_BF16 ? launch_dt<MOMIJ_DTYPE_BF16>(a, grid, warps, smem, nt, gs, vec, stream)
+                                     : launch_dt<MOMIJ_DTYPE_F16>(a, grid, warps, smem, nt, gs, vec, stream);
 }
