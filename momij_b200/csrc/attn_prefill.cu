@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
     __shared__ uint64_t b_q, b_kfull[2], b_kempty[2], b_vfull[2], b_vempty[2], b_s[2], b_p[2][2], b_pv, b_o, b_fin;
     __shared__ uint32_t s_tmem;
     __shared__ float s_m[2][kTileQ], s_l[2][kTileQ];  // of even and odd pages, at the end
-    __shared__ int s_abort, s_last, s_alive[8];
+    __shared__ int s_abort, s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;  // warps 0-7 softmax, 8-15 convert, 16 mma
 
     if (tid == 0) {
@@ -615,9 +615,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
         constexpr int DH = D / 2;                              // this thread's columns of O
         const uint32_t lanes = tmem + tmem_lane_base(warp);
         const uint32_t to = lanes + 256 + e * 128;             // this page kind's O
+        // After a wait that gave up, the pieces that are left pass without work but with
+        // their barriers and counts, so that the workspace stays usable.
         bool ok = true;
         int n = 0, piece = 0;
-        for (int u = u0; u < u1 && ok; ++piece) {
+        for (int u = u0; u < u1; ++piece) {
             const Piece p = piece_at(a, s_pref, u, u1, seg);
             const int J = p.jb - p.ja, rows = p.span.rows, row0 = p.row0, h = p.h;
             const AttnSeq& sq = p.sq;
@@ -673,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             const int all_hi = sq.past + row0 / a.G + 1;
             const int all_lo = a.window > 0 ? sq.past + (row0 + rows - 1) / a.G - a.window + 1 : 0;
             const bool idle = (warp & 3) * 32 >= rows;
-            for (int j = 0; j < J; ++j, ++n) {
+            for (int j = 0; j < J && ok; ++j, ++n) {
                 const int st = n & 1;
                 const uint32_t ts = lanes + st * 128 + e * 64;  // this thread's 64 scores
                 ok = __all_sync(0xffffffffu, wait(&b_s[st], (n >> 1) & 1));
@@ -755,11 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             // ---- results: the two kinds of pages joined, half of the columns a thread -----
             s_m[e][r] = m;
             s_l[e][r] = l;
-            if (lane == 0) s_alive[warp] = ok;
             bar_sync(1, 256);
-            // every warp decides alike whether to go on: they meet again in the next piece
-#pragma unroll
-            for (int k = 0; k < 8; ++k) ok = ok && s_alive[k];
             const float m0 = s_m[0][r], m1 = s_m[1][r];
             m = fmaxf(m0, m1);
             const float w0 = m0 == m ? 1.f : ex2(m0 - m), w1 = m1 == m ? 1.f : ex2(m1 - m);
