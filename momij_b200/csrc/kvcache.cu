@@ -19,11 +19,19 @@
 // stay in registers between the maximum and the coding.  K rows are written
 // as they lie; V is turned through shared memory, so that a page's 64 tokens
 // of one dimension leave as 16-byte stores.  Query heads are spread over the
-// remaining blocks, several heads of a token to a warp, which share the token's
-// weights times cosines and sines.
+// remaining blocks, up to sixteen (D 128) of a token to a warp, which share the
+// token's weights times cosines and sines.
 //
-// What bounds it: bytes (the rows read once, queries and codes written once)
-// for a prompt's chunk, the launch for single tokens.
+// What bounds it: the launch and three dependent reads (length, page, rows) for
+// single tokens (1 token: 3 us, as much for its values); instructions for a
+// prompt's chunk.  4099 tokens of 16 + 2 x 4 heads of 128, 46 MB, with the values
+// read back, 17 MB more: 16.9 us, of which 9 are bytes.  What brought that down
+// from 55: the whole page in one block's registers (27.7), and then half the
+// instructions: packed fp32 arithmetic with registers paired so that a rotation
+// needs no moves, one lane for neighbouring rows so that V turns by byte permutes,
+// all heads of a token in one warp; the raw heads and a page's angles come
+// asynchronously through shared memory, which keeps four blocks on an SM (three:
+// 18.4; two blocks of 512 threads: 21.5).
 #include <algorithm>
 
 #include "host.cuh"
@@ -32,11 +40,27 @@
 namespace momij {
 namespace {
 
-constexpr int kThreads = 256, kWarps = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBlocksPerSm = 4;
 // Pages whose scale would be smaller (values below 7e-18) read as zeros, so that
 // the attention's sums of weights divided by scales stay within fp32.
 constexpr float kMinScale = 0x1p-64f;
-constexpr int kQRows = 4;  // heads per lane group of a query warp
+constexpr int kQRows = 8;  // heads per lane group of a query warp
+
+// Quotient and remainder by a number that the host knows: 2^32 / n rounded down
+// gives a quotient at most one too small for anything below 2^31.
+struct Div {
+    uint32_t n, m;
+    __device__ __forceinline__ int operator()(int x, int& rest) const {
+        uint32_t q = __umulhi((uint32_t)x, m), r = (uint32_t)x - q * n;
+        if (r >= n) {
+            ++q;
+            r -= n;
+        }
+        rest = (int)r;
+        return (int)q;
+    }
+};
+Div div_by(int n) { return Div{(uint32_t)n, 0xffffffffu / (uint32_t)n}; }
 
 struct AppendArgs {
     const uint16_t* qkv;
@@ -49,7 +73,8 @@ struct AppendArgs {
     int32_t* ws;
     const int32_t* stop;
     long long ld;             // elements between token rows of qkv
-    int T, B, Hq, Hkv, n_pages, table_cols, rot, rope_rows, interleaved, touched, kv_blocks, longest, q_chunks;
+    int T, B, Hq, Hkv, n_pages, table_cols, rot, rope_rows, kv_blocks, longest, q_heads;
+    Div by_hkv, by_touched, by_longest, by_split;  // (split: warps a token's query heads are shared by)
     float eps;
 };
 
@@ -87,109 +112,144 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// A head row lies in L = D / 8 lanes, eight elements each.  Norm and rotation
-// are one linear map of the raw row, scaled by its inverse root mean square:
-//   y_j = inv * (x_j * A_j + x'_j * B_j),  A = w cos,  B = +-w' sin
-// with x' (weight w') the element that x_j turns with.  A and B depend on the
-// position alone, so the heads of a token share them.
-struct Turn {
-    float A[8], B[8];
+// Packed fp32 arithmetic: two lanes of a 64-bit register, half the instructions.
+using F2 = uint64_t;
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ F2 f2(float2 v) { return f2(v.x, v.y); }
+__device__ __forceinline__ float2 parts(F2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// A head row lies in L = D / 8 lanes, eight elements each, as four pairs: of
+// neighbours, or with interleaved rotation (IL) of elements two apart, so that x and
+// what it turns with are the same half of two registers.
+template <int DT, bool IL>
+__device__ __forceinline__ void pairs_of(const uint4& v, F2 (&x)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+        const float2 a = unpack<DT>(word(v, k)), b = unpack<DT>(word(v, k + 1));
+        x[k] = IL ? f2(a.x, b.x) : f2(a);
+        x[k + 1] = IL ? f2(a.y, b.y) : f2(b);
+    }
+}
+template <bool IL>
+__device__ __forceinline__ void elements_of(const F2 (&x)[4], float (&e)[8]) {
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+        const float2 a = parts(x[k]), b = parts(x[k + 1]);
+        e[2 * k] = a.x;
+        e[2 * k + 1] = IL ? b.x : a.y;
+        e[2 * k + 2] = IL ? a.y : b.x;
+        e[2 * k + 3] = b.y;
+    }
+}
+// Norm and rotation are one linear map of the raw row, scaled by its inverse root
+// mean square: y_j = inv * (x_j w_j cos + x'_j w'_j (+-sin)), with x' (weight w') the
+// element that x_j turns with.
+//
+// Weights of this lane's elements, and of those they turn with, with sin's sign.
+struct Weights {
+    F2 w[4], p[4];
 };
-template <int DT, int L>
-__device__ __forceinline__ Turn turn_of(const uint16_t* w, const float* table, int rot, int interleaved, int l) {
-    Turn t;
-    const int half = rot >> 1, step = rot >> 4;  // a half's lanes
-    const bool in = 8 * l < rot, first = l < step;
-    const int other = interleaved || !in ? l : first ? l + step : l - step;
-    uint4 g = make_uint4(0u, 0u, 0u, 0u), p = g;
-    if (w) {
-        g = __ldg(reinterpret_cast<const uint4*>(w) + l);
-        p = __ldg(reinterpret_cast<const uint4*>(w) + other);
-    }
+template <int DT, bool IL>
+__device__ __forceinline__ Weights weights_of(const uint16_t* w, int rot, int l) {
+    Weights r;
+    if (!w) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 a = w ? unpack<DT>(word(g, i)) : make_float2(1.f, 1.f);
-        const float2 b = w ? unpack<DT>(word(p, i)) : make_float2(1.f, 1.f);
-        t.A[2 * i] = a.x;
-        t.A[2 * i + 1] = a.y;
-        t.B[2 * i] = interleaved ? b.y : b.x;
-        t.B[2 * i + 1] = interleaved ? b.x : b.y;
-    }
-    if (in) {
-        if (interleaved) {  // pairs (2i, 2i + 1): four angles a lane
-            const float4 cs = __ldg(reinterpret_cast<const float4*>(table + 4 * l));
-            const float4 sn = __ldg(reinterpret_cast<const float4*>(table + half + 4 * l));
-            const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                t.A[j] *= cv[j >> 1];
-                t.B[j] *= j & 1 ? sv[j >> 1] : -sv[j >> 1];
-            }
-        } else {
-            const int i = 8 * (first ? l : l - step);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const float4 cs = __ldg(reinterpret_cast<const float4*>(table + i) + k);
-                const float4 sn = __ldg(reinterpret_cast<const float4*>(table + half + i) + k);
-                const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    t.A[4 * k + j] *= cv[j];
-                    t.B[4 * k + j] *= first ? -sv[j] : sv[j];
-                }
-            }
-        }
+        for (int k = 0; k < 4; ++k) r.w[k] = r.p[k] = f2(1.f, 1.f);
     } else {
+        const int step = rot >> 4;  // a half's lanes
+        pairs_of<DT, IL>(__ldg(reinterpret_cast<const uint4*>(w) + l), r.w);
+        if (!IL) pairs_of<DT, IL>(__ldg(reinterpret_cast<const uint4*>(w) + (l < step ? l + step : l < 2 * step ? l - step : l)), r.p);
+        else
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t.B[j] = 0.f;
+            for (int k = 0; k < 4; ++k) r.p[k] = r.w[k ^ 1];
+    }
+    const float s = l < (rot >> 4) ? -1.f : 1.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (!IL || !(k & 1)) r.p[k] = mul2(r.p[k], IL ? f2(-1.f, -1.f) : f2(s, s));
+    return r;
+}
+// Cosines and sines of this lane's elements at one position (1 and 0 past `rot`).
+struct Angles {
+    F2 c[4], s[4];
+};
+template <bool IL>
+__device__ __forceinline__ Angles angles_of(const float* table, int rot, int l) {
+    Angles t;
+    const int half = rot >> 1, step = rot >> 4;
+    if (8 * l >= rot) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            t.c[k] = f2(1.f, 1.f);
+            t.s[k] = 0;
+        }
+    } else if (IL) {  // pairs (2i, 2i + 1): four angles a lane
+        const float4 c = *reinterpret_cast<const float4*>(table + 4 * l), s = *reinterpret_cast<const float4*>(table + half + 4 * l);
+        t.c[0] = t.c[1] = f2(c.x, c.y);
+        t.c[2] = t.c[3] = f2(c.z, c.w);
+        t.s[0] = t.s[1] = f2(s.x, s.y);
+        t.s[2] = t.s[3] = f2(s.z, s.w);
+    } else {
+        const float4* at = reinterpret_cast<const float4*>(table + 8 * (l < step ? l : l - step));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float4 c = at[k], s = at[half / 4 + k];
+            t.c[2 * k] = f2(c.x, c.y), t.c[2 * k + 1] = f2(c.z, c.w);
+            t.s[2 * k] = f2(s.x, s.y), t.s[2 * k + 1] = f2(s.z, s.w);
+        }
     }
     return t;
 }
-// The turned row; norm: with the inverse root mean square, else 1.
-template <int DT, int L>
-__device__ __forceinline__ void norm_rotate(const uint4& raw, const Turn& t, bool norm, float eps, int rot, int interleaved, int l,
-                                            float (&y)[8]) {
-    float inv = 1.f;
-    if (norm) {
-        float ss = 0.f;
+// The inverse root mean square of a row.
+template <int L>
+__device__ __forceinline__ float inverse_rms(const F2 (&x)[4], float eps) {
+    F2 q = mul2(x[0], x[0]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack<DT>(word(raw, i));
-            ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
-        }
+    for (int i = 1; i < 4; ++i) q = fma2(x[i], x[i], q);
+    const float2 s = parts(q);
+    float ss = s.x + s.y;
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        inv = rsqrtf(ss * (1.f / (8 * L)) + eps);
-    }
-    const int step = rot >> 4;
-    const int src = (threadIdx.x & 31 & ~(L - 1)) + (l < step ? l + step : l < 2 * step ? l - step : l);
+    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    return rsqrtf(ss * (1.f / (8 * L)) + eps);
+}
+// The elements that a lane's turn with: its own, or another lane's.
+template <int DT, bool IL>
+__device__ __forceinline__ void others(const uint4& raw, const F2 (&x)[4], int from, F2 (&o)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t w = word(raw, i);
-        uint32_t o = w;
-        if (rot) o = interleaved ? __byte_perm(w, 0, 0x1032) : __shfl_sync(0xffffffffu, w, src);
-        const float2 f = unpack<DT>(w), q = unpack<DT>(o);
-        y[2 * i] = f.x * t.A[2 * i];
-        y[2 * i + 1] = f.y * t.A[2 * i + 1];
-        if (8 * l < rot) {
-            y[2 * i] = fmaf(q.x, t.B[2 * i], y[2 * i]);
-            y[2 * i + 1] = fmaf(q.y, t.B[2 * i + 1], y[2 * i + 1]);
-        }
-        y[2 * i] *= inv;
-        y[2 * i + 1] *= inv;
-    }
+    for (int k = 0; k < 4; ++k) o[k] = IL ? x[k ^ 1] : f2(unpack<DT>(__shfl_sync(0xffffffffu, word(raw, k), from)));
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
-// Codes 128 + rint(x / scale) of four values: the addition of 1.5 * 2^23 + 128
-// rounds to a whole number (ties to even) and leaves it in the low byte; |x| /
-// scale is at most 127 and a rounding error.  (Of a page with a NaN scale the
-// codes do not matter.)
-__device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
-    uint32_t c[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(fmaf(x[i], inv, 12583040.f));
-    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+// Codes 128 + rint(x / scale): the addition of 1.5 * 2^23 + 128 rounds to a whole
+// number (ties to even) and leaves it in the low byte; |x| / scale is at most 127 and
+// a rounding error.  (Of a page with a NaN scale the codes do not matter.)
+__device__ __forceinline__ F2 coded(F2 x, F2 inv) { return fma2(x, inv, f2(12583040.f, 12583040.f)); }
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040),
+                       0x5410);
+}
+// The largest magnitude; NaN if one is.
+__device__ __forceinline__ float top_of(float m, F2 x) {
+    const float2 v = parts(x);
+    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v.x)), "f"(fabsf(v.y)));
+    return m;
 }
 __device__ __forceinline__ uint32_t recode(uint32_t byte, float ratio) {
     return __float_as_uint(fmaf((float)(int)byte - 128.f, ratio, 12583040.f)) & 255u;
@@ -199,36 +259,38 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
            (recode(w >> 24, ratio) << 24);
 }
 
-template <int DT, int D>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
-    constexpr int L = D / 8, RPW = 32 / L, ROWS = kWarps * RPW;  // lanes a row, rows a warp, rows a sweep
-    constexpr int SWEEPS = kPage / ROWS;
-    constexpr int VP = kPage + 4;  // pitch of the turned V tile
-    __shared__ __align__(16) uint8_t s_v[D * VP];
+template <int DT, int D, bool IL>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) append_kernel(const AppendArgs a) {
+    constexpr int L = D / 8, RPW = 32 / L;      // lanes a row, rows side by side in a warp
+    constexpr int R = kPage / (kWarps * RPW);   // neighbouring rows of a page per lane
+    __shared__ __align__(16) uint32_t s_v[D * kPage / 4];  // the turned V tile: [dimension][row / 4], words swapped about by dimension
+    __shared__ __align__(16) uint4 s_in[kWarps * 32 * kQRows];  // queries: raw heads; keys: the page's rows of the table
     __shared__ uint32_t s_top;
+    static_assert(sizeof(s_in) >= kPage * 128 * 4, "a page's angles");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = lane % L;
     if (tid == 0) s_top = 0;
     pdl_wait();
     const int stopped = __syncthreads_or(tid == 0 && a.stop && __ldcg(a.stop) != 0);
     if (tid == 0 && blockIdx.x == 0 && a.ws) a.ws[kAttnStatus] = stopped ? MOMIJ_ERR_STOPPED : MOMIJ_OK;
     if (stopped) return;
+    const int step = a.rot >> 4;
+    const int from = (lane & ~(L - 1)) + (l < step ? l + step : l < 2 * step ? l - step : l);
 
     if ((int)blockIdx.x >= a.kv_blocks) {
-        // ---- queries: a warp takes RPW * kQRows heads of one token ---------------
-        const int w = (blockIdx.x - a.kv_blocks) * kWarps + warp, t = w / a.q_chunks;
+        // ---- queries: a warp takes q_heads heads of one token, RPW * kQRows at a time ----
+        int part;
+        const int t = a.by_split((blockIdx.x - a.kv_blocks) * kWarps + warp, part);
         if (t >= a.T) return;
-        const int h0 = (w - t * a.q_chunks) * (RPW * kQRows) + lane / L;
-        const uint16_t* src = a.qkv + t * a.ld + 8 * l;
-        uint4 raw[kQRows];
+        const int h0 = part * a.q_heads + lane / L, h1 = min((part + 1) * a.q_heads, a.Hq);
+        const uint16_t* src = a.qkv + t * a.ld + h0 * D + 8 * l;
+        uint4* mine = s_in + warp * (32 * kQRows) + lane;  // (read by the lane that asked for it)
 #pragma unroll
-        for (int i = 0; i < kQRows; ++i) {
-            const int h = h0 + i * RPW;
-            raw[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (h < a.Hq) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + h * D));
-        }
+        for (int i = 0; i < kQRows; ++i)
+            if (h0 + i * RPW < h1) cp_async16(smem_u32(mine + 32 * i), src + i * (RPW * D), true);
+        cp_async_commit();
         const float* table = a.rope;
         if (a.rot) {
-            int b;
+            int b, rest;
             if (a.cu) {  // the sequence whose rows hold t
                 int lo = 0, hi = a.B - 1;
                 while (lo < hi) {
@@ -238,33 +300,59 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
                 }
                 b = lo;
             } else {
-                b = t / a.longest;
+                b = a.by_longest(t, rest);
             }
             const Seq s = sequence(a, b);
-            if (!usable(a, s) || t < s.t0 || t >= s.t0 + s.n) return;  // (reported with the keys)
+            if (!usable(a, s) || t < s.t0 || t >= s.t0 + s.n) {  // (reported with the keys)
+                cp_async_wait<0>();
+                return;
+            }
             table += (long long)(s.past + t - s.t0) * a.rot;
         }
-        const Turn turn = turn_of<DT, L>(a.qw, table, a.rot, a.interleaved, l);
+        F2 A[4], B[4];  // the same for every head
+        {
+            const Weights wt = weights_of<DT, IL>(a.qw, a.rot, l);
+            const Angles an = angles_of<IL>(table, a.rot, l);
 #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                A[i] = mul2(wt.w[i], an.c[i]);
+                B[i] = mul2(wt.p[i], an.s[i]);
+            }
+        }
+        uint16_t* dst = a.q + ((long long)t * a.Hq + h0) * D + 8 * l;
+        cp_async_wait<0>();
+#pragma unroll 2
         for (int i = 0; i < kQRows; ++i) {
-            const int h = h0 + i * RPW;
-            float y[8];
-            norm_rotate<DT, L>(raw[i], turn, a.qw != nullptr, a.eps, a.rot, a.interleaved, l, y);
-            if (h < a.Hq)
-                *reinterpret_cast<uint4*>(a.q + ((long long)t * a.Hq + h) * D + 8 * l) =
-                    make_uint4(pack<DT>(y[0], y[1]), pack<DT>(y[2], y[3]), pack<DT>(y[4], y[5]), pack<DT>(y[6], y[7]));
+            if (part * a.q_heads + i * RPW >= h1) break;
+            const uint4 raw = mine[32 * i];
+            F2 x[4], y[4];
+            pairs_of<DT, IL>(raw, x);
+            const float inv = a.qw ? inverse_rms<L>(x, a.eps) : 1.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = mul2(x[k], A[k]);
+            if (a.rot) {
+                F2 o[4];
+                others<DT, IL>(raw, x, from, o);
+                if (8 * l < a.rot) {  // (past it an infinity would meet a zero)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[k] = fma2(o[k], B[k], y[k]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = mul2(y[k], f2(inv, inv));
+            float e[8];
+            elements_of<IL>(y, e);
+            const uint4 r = make_uint4(pack<DT>(e[0], e[1]), pack<DT>(e[2], e[3]), pack<DT>(e[4], e[5]), pack<DT>(e[6], e[7]));
+            if (h0 + i * RPW < h1) *reinterpret_cast<uint4*>(dst + i * (RPW * D)) = r;
         }
         pdl_launch_dependents();
         return;
     }
 
     // ---- keys or values of one page and head ---------------------------------
-    int u = blockIdx.x;
-    const bool is_v = u & 1;
-    u >>= 1;
-    const int h = u % a.Hkv;
-    u /= a.Hkv;
-    const int j = u % a.touched, b = u / a.touched;
+    int h, j;
+    const bool is_v = blockIdx.x & 1;
+    const int b = a.by_touched(a.by_hkv(blockIdx.x >> 1, h), j);
     const Seq s = sequence(a, b);
     if (!usable(a, s)) {
         if (tid == 0) cache_error(a.ws, MOMIJ_ERR_PAGE);
@@ -274,49 +362,70 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
     const int lo = max(blk * kPage, s.past), hi = min((blk + 1) * kPage, s.past + s.n);  // positions written
     if (lo >= hi) return;
     const int page = blk < a.table_cols ? __ldg(a.table + (long long)b * a.table_cols + blk) : -1;
+    const int r0 = lo - blk * kPage, r1 = hi - blk * kPage;  // rows of the page that are written
+    const int p0 = (warp * RPW + lane / L) * R;              // this lane's first row
+    const uint16_t* src = a.qkv + (long long)(s.t0 + blk * kPage - s.past) * a.ld + (long long)(a.Hq + h + (is_v ? a.Hkv : 0)) * D + 8 * l;
+    uint4 raw[R];  // (on their way while the page is looked up)
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (p0 + i >= r0 && p0 + i < r1) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + (p0 + i) * a.ld));
+    }
+    if (!is_v && a.rot) {  // and the rows' angles, which lie together
+        const float* rows = a.rope + (long long)lo * a.rot;
+        for (int i = tid; i < (hi - lo) * a.rot / 4; i += kThreads) cp_async16(smem_u32(s_in + i), rows + 4 * i, true);
+        cp_async_commit();
+    }
     if (page < 0 || page >= a.n_pages) {
+        cp_async_wait<0>();
         if (tid == 0) cache_error(a.ws, MOMIJ_ERR_PAGE);
         return;
     }
-    const int r0 = lo - blk * kPage, nr = hi - lo;  // first row of the page, rows
     const long long ph = (long long)page * a.Hkv + h;
     float* scale_at = (is_v ? a.vs : a.ks) + ph;
-    const int row_in = warp * RPW + lane / L;  // this lane's row within a sweep
-    const uint16_t* src = a.qkv + (long long)(s.t0 + lo - s.past) * a.ld + (long long)(a.Hq + h + (is_v ? a.Hkv : 0)) * D + 8 * l;
-
     const float had = r0 > 0 ? __ldcg(scale_at) : 0.f;
-    uint4 raw[SWEEPS];
-#pragma unroll
-    for (int i = 0; i < SWEEPS; ++i) {
-        const int r = i * ROWS + row_in;
-        raw[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < nr) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + r * a.ld));
+    const bool busy = (warp + 1) * (RPW * R) > r0 && warp * (RPW * R) < r1;  // the warp has rows to write
+    F2 x[R][4];
+    if (!is_v && a.rot) {
+        cp_async_wait<0>();
+        __syncthreads();
     }
-    float x[SWEEPS][8];
-    uint32_t top = 0;
+    if (busy) {
+        float top = 0.f;
+        if (is_v) {
 #pragma unroll
-    for (int i = 0; i < SWEEPS; ++i) {
-        if (i * ROWS < nr) {
-            const int r = min(i * ROWS + row_in, nr - 1);
-            if (is_v) {
+            for (int i = 0; i < R; ++i) {
+                pairs_of<DT, false>(raw[i], x[i]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float2 f = unpack<DT>(word(raw[i], k));
-                    x[i][2 * k] = f.x;
-                    x[i][2 * k + 1] = f.y;
-                }
-            } else {
-                const Turn turn = turn_of<DT, L>(a.kw, a.rope + (long long)(lo + r) * a.rot, a.rot, a.interleaved, l);
-                norm_rotate<DT, L>(raw[i], turn, a.kw != nullptr, a.eps, a.rot, a.interleaved, l, x[i]);
+                for (int k = 0; k < 4; ++k) top = top_of(top, x[i][k]);  // (rows that are not written: zeros)
             }
-            if (i * ROWS + row_in < nr) {
+        } else {
+            const Weights wt = weights_of<DT, IL>(a.kw, a.rot, l);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) top = max(top, abs_bits(x[i][k]));
+            for (int i = 0; i < R; ++i) {
+                F2 q[4], o[4];
+                pairs_of<DT, IL>(raw[i], q);
+                const float inv = a.kw ? inverse_rms<L>(q, a.eps) : 1.f;
+                if (a.rot) others<DT, IL>(raw[i], q, from, o);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[i][k] = mul2(q[k], wt.w[k]);
+                if (8 * l < a.rot) {
+                    const int row = min(max(p0 + i - r0, 0), r1 - r0 - 1);
+                    const Angles an = angles_of<IL>(reinterpret_cast<const float*>(s_in) + row * a.rot, a.rot, l);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[i][k] = fma2(mul2(o[k], wt.p[k]), an.s[k], mul2(x[i][k], an.c[k]));
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[i][k] = mul2(x[i][k], f2(inv, inv));
+                if (p0 + i >= r0 && p0 + i < r1) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top = top_of(top, x[i][k]);
+                }
             }
         }
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        if (lane == 0 && bits) atomicMax(&s_top, bits);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0 && top) atomicMax(&s_top, top);
     __syncthreads();  // (every thread has read the old scale, too)
     // The scale; infinities and NaN make it NaN, and the page reads as NaN.
     float scale = __uint_as_float(s_top) * (1.f / 127.f);
@@ -326,14 +435,22 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
     const float inv = scale > 0.f ? 1.f / scale : 0.f;
     const bool grew = r0 > 0 && scale > had;  // (false for a NaN scale: its codes do not matter)
     const float ratio = had * inv;
+    const F2 inv2 = f2(inv, inv);
     if (tid == 0) *scale_at = scale;
 
     if (!is_v) {
         uint8_t* dst = a.k + ph * (kPage * D);
+        if (busy) {
 #pragma unroll
-        for (int i = 0; i < SWEEPS; ++i) {
-            const int r = i * ROWS + row_in;
-            if (r < nr) *reinterpret_cast<uint2*>(dst + (r0 + r) * D + 8 * l) = make_uint2(codes4(x[i], inv), codes4(x[i] + 4, inv));
+            for (int i = 0; i < R; ++i) {
+                if (p0 + i < r0 || p0 + i >= r1) continue;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[i][k] = coded(x[i][k], inv2);
+                float e[8];
+                elements_of<IL>(x[i], e);
+                *reinterpret_cast<uint2*>(dst + (p0 + i) * D + 8 * l) =
+                    make_uint2(low_bytes(e[0], e[1], e[2], e[3]), low_bytes(e[4], e[5], e[6], e[7]));
+            }
         }
         if (grew)
             for (int i = tid; i < r0 * D / 4; i += kThreads) {
@@ -341,37 +458,53 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
                 *p = recode4(*p, ratio);
             }
     } else {
+        // Word w of dimension d lies at d * 16 + (w ^ (d / 8 & 15)): lanes that store
+        // one k together differ in d / 8, and a reader takes four whole words.
         uint8_t* dst = a.v + ph * (kPage * D);
+        if (busy) {
 #pragma unroll
-        for (int i = 0; i < SWEEPS; ++i) {
-            const int r = i * ROWS + row_in;
-            if (r < nr) {
-                uint8_t* t = s_v + 8 * l * VP + r0 + r;
+            for (int k = 0; k < 4; ++k) {
+                float2 v[R];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t c = codes4(x[i] + 4 * k, inv);
+                for (int i = 0; i < R; ++i) v[i] = parts(coded(x[i][k], inv2));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) t[(4 * k + e) * VP] = (uint8_t)(c >> (8 * e));
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t* at = s_v + (8 * l + 2 * k + e) * 16 + ((p0 >> 2) ^ (l & 15));
+                    const uint32_t c = low_bytes(e ? v[0].y : v[0].x, e ? v[1].y : v[1].x, e ? v[R / 2].y : v[R / 2].x, e ? v[R - 1].y : v[R - 1].x);
+                    if (R == 4) *at = c;
+                    else reinterpret_cast<uint16_t*>(at)[(p0 >> 1) & 1] = (uint16_t)c;
                 }
             }
         }
         __syncthreads();
-        const int r1 = r0 + nr, w0 = grew ? 0 : r0;  // rows [w0, r1) change
+        const int w0 = grew ? 0 : r0;  // rows [w0, r1) change
         for (int i = tid; i < D * (kPage / 16); i += kThreads) {
             const int d = i >> 2, c0 = (i & 3) * 16, c1 = c0 + 16;
             if (c1 <= w0 || c0 >= r1) continue;
             uint8_t* p = dst + d * kPage + c0;
-            const uint8_t* t = s_v + d * VP + c0;
+            uint32_t t[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[k] = s_v[d * 16 + (((c0 >> 2) + k) ^ ((d >> 3) & 15))];
             if (c0 >= r0 && c1 <= r1) {  // all new
-                const uint32_t* tw = reinterpret_cast<const uint32_t*>(t);
-                *reinterpret_cast<uint4*>(p) = make_uint4(tw[0], tw[1], tw[2], tw[3]);
+                *reinterpret_cast<uint4*>(p) = make_uint4(t[0], t[1], t[2], t[3]);
             } else {
-                for (int e = max(0, w0 - c0); e < min(16, r1 - c0); ++e)
-                    p[e] = c0 + e >= r0 ? t[e] : (uint8_t)recode(p[e], ratio);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (c0 + e >= w0 && c0 + e < r1) p[e] = c0 + e >= r0 ? (uint8_t)(t[e >> 2] >> (8 * (e & 3))) : (uint8_t)recode(p[e], ratio);
             }
         }
     }
     pdl_launch_dependents();
+}
+
+template <int DT>
+int append_launch(dim3 grid, int D, bool interleaved, const AppendArgs& a, momij_stream_t stream) {
+    const dim3 block(kThreads);
+    if (D == 64)
+        return interleaved ? host_launch(append_kernel<DT, 64, true>, grid, block, 0, stream, a)
+                           : host_launch(append_kernel<DT, 64, false>, grid, block, 0, stream, a);
+    return interleaved ? host_launch(append_kernel<DT, 128, true>, grid, block, 0, stream, a)
+                       : host_launch(append_kernel<DT, 128, false>, grid, block, 0, stream, a);
 }
 
 struct ReadArgs {
@@ -381,7 +514,8 @@ struct ReadArgs {
     uint16_t *ko, *vo;
     int32_t* ws;
     const int32_t* stop;
-    int B, Hkv, n_pages, table_cols, count, parts;
+    int B, Hkv, n_pages, table_cols, count;
+    Div by_hkv, by_parts;
 };
 
 // Values of `count` tokens from first[b] on as [B, count, Hkv, D]; a token at
@@ -389,19 +523,15 @@ struct ReadArgs {
 // of one head; tokens need not start at a page.
 template <int DT, int D>
 __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
-    constexpr int VP = kPage + 4;
-    __shared__ __align__(16) uint8_t s_v[D * VP];
+    __shared__ __align__(16) uint32_t s_v[D * kPage / 4];  // as in append_kernel
     const int tid = threadIdx.x;
     pdl_wait();
     const int stopped = __syncthreads_or(tid == 0 && a.stop && __ldcg(a.stop) != 0);
     if (tid == 0 && blockIdx.x == 0 && a.ws) a.ws[kAttnStatus] = stopped ? MOMIJ_ERR_STOPPED : MOMIJ_OK;
     if (stopped) return;
-    int u = blockIdx.x;
-    const bool is_v = u & 1;
-    u >>= 1;
-    const int h = u % a.Hkv;
-    u /= a.Hkv;
-    const int j = u % a.parts, b = u / a.parts;
+    int h, j;
+    const bool is_v = blockIdx.x & 1;
+    const int b = a.by_parts(a.by_hkv(blockIdx.x >> 1, h), j);
     const long long from = a.first ? __ldg(a.first + b) : 0;
     const int len = __ldg(a.lens + b);
     if (from < 0) {
@@ -422,39 +552,58 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
     const long long ph = (long long)(page < 0 ? 0 : page) * a.Hkv + h;
     const float scale = page < 0 ? 0.f : __ldg((is_v ? a.vs : a.ks) + ph);
     const uint8_t* src = (is_v ? a.v : a.k) + ph * (kPage * D);
-    if (is_v && page >= 0) {
+    uint16_t* out = (is_v ? a.vo : a.ko) + ((long long)b * a.count * a.Hkv + h) * D;
+    constexpr int L = D / 8, RPW = 32 / L, R = kPage / (kWarps * RPW);
+    const int l = tid % L, r = tid / L * R;  // this thread's eight dimensions, and R neighbouring rows
+    uint32_t c[R][2];                        // their codes
+    if (!is_v) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const uint2 w = page >= 0 ? __ldg(reinterpret_cast<const uint2*>(src + (r + i) * D + 8 * l)) : make_uint2(0u, 0u);
+            c[i][0] = w.x;
+            c[i][1] = w.y;
+        }
+    } else if (page >= 0) {
         for (int i = tid; i < D * (kPage / 16); i += kThreads) {
-            const int d = i >> 2, c0 = (i & 3) * 16;
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + d * kPage + c0));
-            uint32_t* t = reinterpret_cast<uint32_t*>(s_v + d * VP + c0);
-            t[0] = w.x;
-            t[1] = w.y;
-            t[2] = w.z;
-            t[3] = w.w;
+            const int d = i >> 2, c0 = (i & 3) * 4;
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(src) + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s_v[d * 16 + ((c0 + k) ^ ((d >> 3) & 15))] = word(w, k);
         }
         __syncthreads();
-    }
-    uint16_t* out = (is_v ? a.vo : a.ko) + ((long long)b * a.count * a.Hkv + h) * D;
-    constexpr int L = D / 8;
+        uint32_t w[8];  // a dimension's rows, this thread's first in the low byte
 #pragma unroll
-    for (int i = tid; i < kPage * L; i += kThreads) {
-        const int r = i / L, l = i % L;
-        const long long t = p0 + r;
+        for (int e = 0; e < 8; ++e) w[e] = s_v[(8 * l + e) * 16 + ((r >> 2) ^ (l & 15))] >> (8 * (r & 3));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {  // bytes of four dimensions turned into rows
+            const uint32_t a01 = __byte_perm(w[4 * k], w[4 * k + 1], 0x5140), a23 = __byte_perm(w[4 * k + 2], w[4 * k + 3], 0x5140);
+            c[0][k] = __byte_perm(a01, a23, 0x5410);
+            c[1][k] = __byte_perm(a01, a23, 0x7632);
+            if (R == 4) {
+                const uint32_t b01 = __byte_perm(w[4 * k], w[4 * k + 1], 0x7362), b23 = __byte_perm(w[4 * k + 2], w[4 * k + 3], 0x7362);
+                c[R - 2][k] = __byte_perm(b01, b23, 0x5410);
+                c[R - 1][k] = __byte_perm(b01, b23, 0x7632);
+            }
+        }
+    }
+    const F2 scale2 = f2(scale, scale);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const long long t = p0 + r + i;
         if (t < t0 || t >= t1) continue;
         uint4 o = make_uint4(0u, 0u, 0u, 0u);
         if (t < len) {
-            uint2 c;
-            if (is_v) {
-                const uint8_t* q = s_v + 8 * l * VP + r;
-                c.x = q[0] | ((uint32_t)q[VP] << 8) | ((uint32_t)q[2 * VP] << 16) | ((uint32_t)q[3 * VP] << 24);
-                c.y = q[4 * VP] | ((uint32_t)q[5 * VP] << 8) | ((uint32_t)q[6 * VP] << 16) | ((uint32_t)q[7 * VP] << 24);
-            } else {
-                c = __ldg(reinterpret_cast<const uint2*>(src + r * D + 8 * l));
-            }
-            float f[8];
+            uint32_t y[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = ((float)(int)(((e < 4 ? c.x : c.y) >> (8 * (e & 3))) & 255u) - 128.f) * scale;
-            o = make_uint4(pack<DT>(f[0], f[1]), pack<DT>(f[2], f[3]), pack<DT>(f[4], f[5]), pack<DT>(f[6], f[7]));
+            for (int k = 0; k < 4; ++k) {
+                // a code in the low byte of 2^23: the subtraction is exact
+                const uint32_t w = c[i][k >> 1];
+                const float a0 = __uint_as_float(__byte_perm(w, 0x4b000000u, k & 1 ? 0x7442 : 0x7440)) - 8388736.f;
+                const float a1 = __uint_as_float(__byte_perm(w, 0x4b000000u, k & 1 ? 0x7443 : 0x7441)) - 8388736.f;
+                const float2 v = parts(mul2(f2(a0, a1), scale2));
+                y[k] = pack<DT>(v.x, v.y);
+            }
+            o = make_uint4(y[0], y[1], y[2], y[3]);
         }
         *reinterpret_cast<uint4*>(out + (t - from) * ((long long)a.Hkv * D) + 8 * l) = o;
     }
@@ -508,23 +657,27 @@ extern "C" int momij_qk_norm_rope_append(const void* qkv, long long ld, void* q_
     a.table_cols = table_cols;
     a.rot = rot;
     a.rope_rows = rope_rows;
-    a.interleaved = interleaved != 0;
     a.eps = eps;
     const int longest = cu_q ? (max_q > 0 ? std::min(max_q, T) : T) : T / B;
     a.longest = longest;
-    a.touched = (longest + kPage - 2) / kPage + 1;  // pages a sequence's new tokens can touch
-    const long long kv = (long long)B * a.touched * Hkv * 2;
-    const int heads = (256 / D) * kQRows;  // of one token, per warp
-    a.q_chunks = (Hq + heads - 1) / heads;
-    const long long blocks = kv + ((long long)T * a.q_chunks + kWarps - 1) / kWarps;
-    if (blocks > 0x7fffffffLL) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
+    const int touched = (longest + kPage - 2) / kPage + 1;  // pages a sequence's new tokens can touch
+    const long long kv = (long long)B * touched * Hkv * 2;
+    // Query heads of a token: as many to a warp as it can hold (a token's weights and
+    // angles are half of a warp's instructions), fewer while there is room for more warps.
+    const int rows = 256 / D;
+    a.q_heads = rows * kQRows;
+    while (a.q_heads > rows && (long long)T * ((Hq + a.q_heads / 2 - 1) / (a.q_heads / 2)) <= kBlocksPerSm * kWarps * host_sm_count()) a.q_heads /= 2;
+    const int warps = (Hq + a.q_heads - 1) / a.q_heads;
+    a.by_hkv = div_by(Hkv);
+    a.by_touched = div_by(touched);
+    a.by_longest = div_by(longest);
+    a.by_split = div_by(warps);
+    const long long blocks = kv + ((long long)T * warps + kWarps - 1) / kWarps;
+    if (blocks > 0x7fffffffLL || (long long)T * warps > 0x7ffffff0LL) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     a.kv_blocks = (int)kv;
-    const dim3 grid((unsigned)blocks), block(kThreads);
-    if (dtype == MOMIJ_DTYPE_BF16)
-        return D == 64 ? host_launch(append_kernel<MOMIJ_DTYPE_BF16, 64>, grid, block, 0, stream, a)
-                       : host_launch(append_kernel<MOMIJ_DTYPE_BF16, 128>, grid, block, 0, stream, a);
-    return D == 64 ? host_launch(append_kernel<MOMIJ_DTYPE_F16, 64>, grid, block, 0, stream, a)
-                   : host_launch(append_kernel<MOMIJ_DTYPE_F16, 128>, grid, block, 0, stream, a);
+    const dim3 grid((unsigned)blocks);
+    return dtype == MOMIJ_DTYPE_BF16 ? append_launch<MOMIJ_DTYPE_BF16>(grid, D, interleaved != 0, a, stream)
+                                     : append_launch<MOMIJ_DTYPE_F16>(grid, D, interleaved != 0, a, stream);
 }
 
 extern "C" int momij_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_scales, const float* v_scales,
@@ -557,8 +710,10 @@ extern "C" int momij_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, 
     a.n_pages = n_pages;
     a.table_cols = table_cols;
     a.count = count;
-    a.parts = first ? (count + kPage - 2) / kPage + 1 : (count + kPage - 1) / kPage;
-    const long long blocks = (long long)B * a.parts * Hkv * 2;
+    const int parts = first ? (count + kPage - 2) / kPage + 1 : (count + kPage - 1) / kPage;
+    a.by_hkv = div_by(Hkv);
+    a.by_parts = div_by(parts);
+    const long long blocks = (long long)B * parts * Hkv * 2;
     if (blocks > 0x7fffffffLL) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     const dim3 grid((unsigned)blocks), block(kThreads);
     if (dtype == MOMIJ_DTYPE_BF16)
