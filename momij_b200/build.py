@@ -22,7 +22,7 @@ OBJ = os.path.join(HERE, "_build")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libmomij_moe.so")
 SOURCES = ["route.cu", "gemv.cu", "layer.cu", "token.cu", "decode.cu", "block.cu", "prefill.cu", "ep.cu", "ep_host.cu", "misc.cu",
-           "api.cu", "noalloc.cu", "kvcache.cu", "attn.cu", "attn_prefill.cu", "qmm4.cu", "logits.cu"]
+           "api.cu", "noalloc.cu", "kvcache.cu", "attn.cu", "attn_prefill.cu", "qmm4.cu", "qmm4_tc.cu", "logits.cu"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -1,7 +1,9 @@
 // qmm4.cu -- products of a few tokens with a 4-bit weight matrix:
 //   y[m, n] = sum_k (s[n, k/gs] * q[n, k] + b[n, k/gs]) * x[m, k],  q in 0..15,
 // for attention projections and the vocabulary projection (momij
-// QuantProj.swift; SeedlessMetal.swift:2598-2716 for the 4-bit output head).
+// QuantProj.swift; SeedlessMetal.swift:2598-2716 for the 4-bit output head).  This
+// kernel serves one and few tokens and small matrices; qmm4_tc.cu has the other and
+// the rule between them.
 //
 // Mathematics.  Per scale group the product splits into s * sum(q x) and
 // b * sum(x): the inner sum runs on the tensor cores (mma.sync m16n8k16, fp32
@@ -25,7 +27,7 @@
 // registers left room for 24 warps with 3 KB each in flight.)
 #include <algorithm>
 
-#include "host.cuh"
+#include "qmm4.cuh"
 
 namespace momij {
 namespace {
@@ -59,19 +61,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-// The two 16-bit values of a word as floats.
-template <int DT>
-__device__ __forceinline__ float half_of(uint32_t w, int hi) {
-    if (DT == MOMIJ_DTYPE_BF16) return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
-    return Half<DT>::to_f((uint16_t)(hi ? w >> 16 : w & 0xffffu));
-}
-
 // ONE: a pass of a single token, which is column 0.  VEC: a batch's scales of a
 // row are one aligned copy; otherwise they are read where they are used.
 template <int DT, int NT, int GS, bool VEC, bool ONE>
@@ -139,14 +128,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) qmm4_kernel(const Args a) {
     // largest), then the permuted fp16 operand and the group sums; the pieces of
     // all tokens in one line ----------------------------------------------------
     const int nc = a.K / 8, np = mt * nc;  // 8-element pieces per token, in all
-    auto piece = [&](int m, int p) -> uint4 {
-        const uint16_t* src = a.x + (m0 + m) * a.ldx + 8 * p;
-        if (a.xvec) return __ldg(reinterpret_cast<const uint4*>(src));
-        uint32_t v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __ldg(src + 2 * i) | ((uint32_t)__ldg(src + 2 * i + 1) << 16);
-        return make_uint4(v[0], v[1], v[2], v[3]);
-    };
+    auto piece = [&](int m, int p) { return qmm4_piece(a.x + (m0 + m) * a.ldx + 8 * p, a.xvec); };
     for (int i0 = 0; i0 < np; i0 += 2 * threads) {
         uint4 v[2];
         int m[2];
@@ -160,10 +142,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) qmm4_kernel(const Args a) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             if (i0 + k * threads + (warp << 5) >= np) break;
-            const uint32_t t[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = max(top, max(t[i] & 0x7fffu, (t[i] >> 16) & 0x7fffu));
+            uint32_t top = qmm4_top(v[k]);
             const int first = __shfl_sync(0xffffffffu, m[k], 0);  // most warps hold one token's pieces
             if (ONE || __all_sync(0xffffffffu, m[k] == first)) {
                 top = __reduce_max_sync(0xffffffffu, top);
@@ -174,13 +153,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) qmm4_kernel(const Args a) {
         }
     }
     __syncthreads();
-    // A token's biased exponent, from which x is scaled so that its largest
-    // magnitude becomes 2^14 .. 2^15; 141 (a factor of one) for zeros, infinities and
-    // NaN.  Tokens below 2^-112 stay smaller.
-    auto exponent = [&](int m) -> int {
-        const uint32_t u = __float_as_uint(Half<DT>::to_f((uint16_t)s_e[m]));
-        return u == 0 || u >= 0x7f800000u ? 141 : max((int)(u >> 23), 15);
-    };
+    auto exponent = [&](int m) { return qmm4_exponent<DT>(s_e[m]); };
     for (int i0 = 0; i0 < np; i0 += 2 * threads) {
         uint4 v[2];
         int m[2];
@@ -196,29 +169,16 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) qmm4_kernel(const Args a) {
             const int i = i0 + k * threads + tid, p = i - m[k] * nc;
             if (i0 + k * threads + (warp << 5) >= np) break;
             const float f = __uint_as_float((uint32_t)(268 - exponent(m[k])) << 23);
-            const uint32_t t[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-            float e[8], sum = 0.f;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                e[2 * q] = half_of<DT>(t[q], 0) * f;
-                e[2 * q + 1] = half_of<DT>(t[q], 1) * f;
-            }
-#pragma unroll
-            for (int q = 0; q < 8; ++q) sum += e[q];
+            float sum;
+            const uint4 o = qmm4_operand<DT>(v[k], f, sum);
             if (i < np) {
-                uint4 o;
-                o.x = f16x2(e[0], e[4]);
-                o.y = f16x2(e[1] * 0.0625f, e[5] * 0.0625f);
-                o.z = f16x2(e[2], e[6]);
-                o.w = f16x2(e[3] * 0.0625f, e[7] * 0.0625f);
                 // piece p = (block, lane c, word j): the lane's pieces of one word lie side by side
                 const int blk = p >> 3, pc = (p >> 1) & 3, j = p & 1;
                 *reinterpret_cast<uint4*>(sx + m[k] * a.pitch + blk * 128 + j * 64 + pc * 16) = o;
             }
 #pragma unroll
             for (int o = 1; o < GS / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            // 2^-24: the unit of the codes' products
-            if (i < np && (p & (GS / 8 - 1)) == 0) xs[(p / (GS / 8)) * (8 * NT) + m[k]] = sum * 5.9604644775390625e-08f;
+            if (i < np && (p & (GS / 8 - 1)) == 0) xs[(p / (GS / 8)) * (8 * NT) + m[k]] = sum * kQmm4Unit;
         }
     }
     __syncthreads();
@@ -371,6 +331,9 @@ extern "C" int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const
         return MOMIJ_ERR_INVALID_ARGUMENT;
     const int sms = host_sm_count();
     if (sms <= 0) return MOMIJ_ERR_CUDA;
+    const Qmm4Call call{static_cast<const uint16_t*>(x), w, static_cast<const uint16_t*>(scales), static_cast<const uint16_t*>(biases),
+                        static_cast<uint16_t*>(y), ldx, ldy, M, N, K, gs, dtype};
+    if (qmm4_tc_takes(call)) return qmm4_tc_launch(call, stream);
 
     Args a{};
     a.x = static_cast<const uint16_t*>(x);

@@ -133,6 +133,91 @@ def test_qmm4_stream_graph_and_refusals():
     assert e.value.status == moe.INVALID_ARGUMENT
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K,gs", [
+    (2, 128, 256, 64), (2, 129, 320, 64), (3, 1000, 1088, 64), (9, 5000, 384, 128), (16, 300, 2048, 64), (17, 257, 640, 128), (32, 4100, 2112, 64),
+    (33, 513, 4096, 128), (20, 20000, 1024, 64), (7, 2500, 12800, 128), (32, 640, 8192, 64), (30, 130, 14336, 128)])
+def test_qmm4_several_tokens_match_64_bits(M, N, K, gs, dtype):
+    """Sizes with a last tile, batch and token group that are not full, matrices of
+    few rows and many columns (shared by several blocks), many rounds of tiles."""
+    w, s, b = weights(N, K, gs, dtype, 11)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(12)).to(R.TD[dtype])
+    y = head.qmm4(x.cuda(), w.cuda(), s.cuda(), b.cuda(), gs=gs)
+    check_qmm4(y, x, w, s, b, gs)
+    again = head.qmm4(x.cuda(), w.cuda(), s.cuda(), b.cuda(), gs=gs)
+    assert torch.equal(y, again)
+
+
+@pytest.mark.parametrize("M", [2, 18])
+@pytest.mark.parametrize("off", [0, 1, 3])
+def test_qmm4_several_tokens_strides_and_alignment(M, off):
+    N, K, gs = 200, 1024, 64
+    w, s, b = weights(N, K, gs, "bf16", 13)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(14)).bfloat16()
+    ref = head.qmm4(x.cuda(), w.cuda(), s.cuda(), b.cuda(), gs=gs)
+    check_qmm4(ref, x, w, s, b, gs)
+    wide = torch.zeros(M, K + 24, dtype=x.dtype, device="cuda")
+    wide[:, off:off + K] = x.cuda()
+    views = []
+    for t in (s, b):
+        f = torch.zeros(t.numel() + 8, dtype=t.dtype, device="cuda")
+        f[off:off + t.numel()] = t.cuda().flatten()
+        views.append(f[off:off + t.numel()].view(t.shape))
+    out = torch.full((M, N + 5), 9.0, dtype=x.dtype, device="cuda")
+    y = head.qmm4(wide[:, off:off + K], w.cuda(), *views, gs=gs, out=out[:, 2:2 + N])
+    assert torch.equal(y, ref) and (out[:, :2] == 9).all() and (out[:, 2 + N:] == 9).all()
+
+
+def test_qmm4_several_tokens_magnitudes():
+    N, K, gs = 150, 512, 64
+    w, s, b = weights(N, K, gs, "bf16", 15)
+    g = torch.Generator().manual_seed(16)
+    x = (torch.randn(6, K, generator=g) * torch.tensor([1.0, 2.0 ** 90, 2.0 ** -90, 0.0, 1.0, 1.0])[:, None]).bfloat16()
+    x[4, 3], x[5, 400] = math.inf, math.nan
+    y = head.qmm4(x.cuda(), w.cuda(), s.cuda(), b.cuda(), gs=gs)
+    check_qmm4(y[:4], x[:4], w, s, b, gs)
+    assert (y[3] == 0).all() and not torch.isfinite(y[4:]).any()
+
+
+def test_qmm4_matrix_past_32_bits_several_tokens():
+    N, K, gs = 2_150_000, 4096, 128
+    w = torch.zeros(N, K // 8, dtype=torch.int32, device="cuda")
+    s = torch.zeros(N, K // gs, dtype=torch.bfloat16, device="cuda")
+    b = torch.zeros(N, K // gs, dtype=torch.bfloat16, device="cuda")
+    wt, st, bt = weights(40, K, gs, "bf16", 3)
+    w[-40:], s[-40:], b[-40:] = wt.cuda(), st.cuda(), bt.cuda()
+    x = torch.randn(3, K, generator=torch.Generator().manual_seed(8)).bfloat16()
+    y = head.qmm4(x.cuda(), w, s, b, gs=gs)
+    check_qmm4(y[:, -40:], x, wt, st, bt, gs)
+    assert (y[:, :-40] == 0).all()
+
+
+def test_qmm4_stop_flag_and_wait_limit():
+    """A raised stop flag leaves the output as it was; waits that give up at once show
+    as NaN or not at all, and the next call is right."""
+    w, s, b = (t.cuda() for t in weights(3000, 2048, 64, "bf16", 17))
+    x = torch.randn(12, 2048, device="cuda").bfloat16()
+    ref = head.qmm4(x, w, s, b)
+    out = torch.full_like(ref, 5.0)
+    flag = torch.ones(1, dtype=torch.int32, device="cuda")
+    moe.set_stop_flag(flag)
+    try:
+        head.qmm4(x, w, s, b, out=out)
+        torch.cuda.synchronize()
+    finally:
+        moe.set_stop_flag(None)
+    assert (out == 5).all()
+    moe.set_spin_limit(-1)
+    try:
+        head.qmm4(x, w, s, b, out=out)
+        torch.cuda.synchronize()
+    finally:
+        moe.set_spin_limit(0)
+    assert bool((torch.isnan(out) | (out == ref)).all())
+    for _ in range(2):
+        assert torch.equal(head.qmm4(x, w, s, b), ref)
+
+
 # ---- logits -----------------------------------------------------------------------------
 
 def check_logits(out, ref, size):
