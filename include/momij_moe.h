@@ -311,8 +311,9 @@ size_t momij_attention_workspace_size(int T, int Hq);
  * positions p - window < j <= p of the token's sequence (window 0: all), with
  * p = lens[b] - n_b + i for its i-th new token; kv head hq / (Hq / Hkv).  A row
  * that sees no position (lens[b] < n_b) gives zeros.  Rows of q and out are ldq
- * and ldo elements apart (ldo % 4 == 0).  One launch; the result does not depend
- * on scheduling.
+ * and ldo elements apart (ldo % 4 == 0).  One launch, or a second that joins what
+ * blocks share (more than 16 rows per kv head, few heads); the result does not
+ * depend on scheduling.
  * Replaces: the 16-bit attention of SeedlessMetal.swift:2794-3004. */
 int momij_attention(const void* q, long long ldq, void* out, long long ldo, const uint8_t* k_codes,
                     const uint8_t* v_codes, const float* k_scales, const float* v_scales, int n_pages,
@@ -324,7 +325,9 @@ int momij_attention(const void* q, long long ldq, void* out, long long ldo, cons
  * (MLX affine, transpose=true): w uint32 [N, K/8], code k at bits [4(k%8),
  * 4(k%8)+3]; s, b 16-bit [N, K/gs], gs 64 or 128, K % gs == 0; w 16-byte aligned.
  * Rows of x and y are ldx and ldy elements apart.  For few tokens: up to 32 share
- * a pass over the matrix (fewer for K above 3,000 or so).
+ * a pass over the matrix, one launch each (fewer for K above 14,000 or so).  The call
+ * has no workspace: a raised stop flag leaves y as it was, and a device-side wait that
+ * gave up leaves NaN in the tile it was for.
  * Replaces: the 4-bit output head's product (SeedlessMetal.swift:2598-2716) and
  * MLX.quantizedMM of 4-bit projections (QuantProj.swift). */
 int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const void* scales, const void* biases, void* y,
@@ -339,7 +342,8 @@ int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const void* scal
  * history int32 [n_history], row b's ids at cu_history[b] .. cu_history[b+1]-1;
  * bias_ids and bias [n_bias] by cu_bias alike, the last entry of a token holds;
  * ids outside [0, V) are skipped.  Any of the inputs may be NULL (no history,
- * repetition 1, presence and frequency 0, no bias, no mask).
+ * repetition 1, presence and frequency 0, no bias, no mask).  out may be logits
+ * itself where that is fp32 with ld == V.  One launch, two for large batches.
  * Replaces: LogitsProcessor.swift's penalties and XGrammarGuide.swift's mask. */
 int momij_process_logits(const void* logits, long long ld, int dtype, float* out, int B, int V,
                          const int32_t* history, const int32_t* cu_history, int n_history, const float* repetition,
