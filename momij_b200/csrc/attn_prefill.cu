@@ -693,6 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
                 const float iv = sc[2];
                 const int t0 = (first_page + 2 * j + e) * kPage;
                 tmem_ld_wait();
+                settle(*reinterpret_cast<uint32_t(*)[kPage]>(s));
                 if (t0 + kPage > all_hi || t0 < all_lo) {  // some row does not see all of the page
 #pragma unroll
                     for (int i = 0; i < kPage; ++i) {
@@ -723,6 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
                             uint32_t v[16];
                             tmem_ld16_nowait(to + 16 * c, v);
                             tmem_ld_wait();
+                            settle(v);
 #pragma unroll
                             for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
                             tmem_st16(to + 16 * c, v);
@@ -772,6 +774,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
                     tmem_ld16_nowait(lanes + 256 + e * DH + 16 * c, v);
                     tmem_ld16_nowait(lanes + 384 + e * DH + 16 * c, y);
                     tmem_ld_wait();
+                    settle(v);
+                    settle(y);
                     if (!mine) continue;
                     // one kind's O holds nothing when none of its pages was seen: its weight is zero then
                     float o[16];

@@ -16,15 +16,16 @@
 // block's shared memory (two tiles' worth of room), where two warps add them in rank
 // order while the next tile is under way.
 //
-// What bounds it: the eight summing warps (a warp's chain of accumulator reads, group
-// sums and scales takes about 1,000 cycles a batch of 16 or 32 tokens) and behind them
-// the conversion (16 KB of codes cost 16 x 100 instructions); a batch's bytes would come
-// in 750 cycles.  The tensor pipe is busy a tenth of the time.  151,936 x 2,048: 9
-// tokens 47 us, 32 tokens 63 us (155 with the other kernel), 26 for the bytes alone;
-// 20,000 x 6,400: 29 and 39 (49 and 152).
+// What bounds it: the eight summing warps (a chain of accumulator reads, group sums and
+// scales a batch) and close behind them the conversion (16 KB of codes and their scales
+// cost 16 x 120 instructions); a batch's bytes would come in 750 cycles.  The tensor
+// pipe is busy a tenth of the time.  151,936 x 2,048: 9 tokens 45 us, 32 tokens 58 us
+// (155 with the other kernel), 26 for the bytes alone; 20,000 x 6,400: 29 and 37 (49
+// and 152).
 // What brought it there: partial sums sent asynchronously and finished by warps of their
 // own (79 us; a releasing arrival per warp costs a microsecond a tile), two sets of
-// converting warps that take batches in turn (51.6), packed sums.
+// converting warps that take batches in turn (51.6), packed sums, scales fetched by the
+// converting warps (47; 63 for 32 tokens).
 #include <algorithm>
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -41,6 +42,7 @@ constexpr int kConv = 16, kEpi = 8, kFin = 2;                 // warps
 constexpr int kEpiWarp = kConv, kMmaWarp = kConv + kEpi, kTmaWarp = kMmaWarp + 1, kFinWarp = kTmaWarp + 1;
 constexpr int kThreads = 32 * (kFinWarp + kFin);
 constexpr int kMaxStages = 6, kMinStages = 3;
+constexpr int kScaleRing = 8;  // batches: a row's scales are written when the sums of five batches ago are through
 constexpr size_t kBudget = 224 * 1024;
 
 struct TcArgs {
@@ -94,13 +96,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
-}
-
-// Values that a wait has made valid: nothing that uses them moves before this.
-template <int N>
-__device__ __forceinline__ void settle(uint32_t (&v)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
 }
 
 // ---- cluster ---------------------------------------------------------------------
@@ -166,7 +161,8 @@ __global__ void __launch_bounds__(kThreads, 1) qmm4_tc_kernel(const __grid_const
     // ring | x | group sums | exchange
     unsigned char* sx = sm + a.stages * kStage;
     float* s_sum = reinterpret_cast<float*>(sx + a.cap * (kCols / 64) * ATOM);       // [group][NT]
-    float* s_part = s_sum + a.cap * GPB * NT;                                        // [2][S][row][PITCH]
+    uint32_t* s_sb = reinterpret_cast<uint32_t*>(s_sum + a.cap * GPB * NT);          // [batch % 8][group][row]: scale, bias
+    float* s_part = reinterpret_cast<float*>(s_sb + kScaleRing * GPB * kRows);       // [2][S][row][PITCH]
     const int b0 = (int)((long long)a.nbatch * rank / S), nb = (int)((long long)a.nbatch * (rank + 1) / S) - b0;  // this block's batches
     const int k0 = b0 * kCols, kw = min(a.K - k0, nb * kCols);                       // its columns
 
@@ -364,6 +360,33 @@ __global__ void __launch_bounds__(kThreads, 1) qmm4_tc_kernel(const __grid_const
         const int total = cl < a.tiles ? ((a.tiles - cl + ncl - 1) / ncl) * nb : 0;
         int st = warp >> 3, ua = st;
         uint32_t ph = 0, pa = 1;
+        // This row's scales and biases of the warp's groups, one batch of the warp ahead.
+        constexpr int GW = GPB / 2;
+        const int ng = a.K / GS;
+        uint32_t sv = 0, bv = 0;
+        int lt = cl, lj = warp >> 3;
+        auto fetch = [&]() {
+            while (lj >= nb) {
+                lj -= nb;
+                lt += ncl;
+            }
+            if (lt >= a.tiles) return;
+            const int g = (b0 + lj) * GPB + kp * GW;
+            const long long at = (long long)min(lt * kRows + r, a.N - 1) * ng + g;
+            if (GW == 2 && a.svec) {
+                sv = g < ng ? __ldg(reinterpret_cast<const uint32_t*>(a.s + at)) : 0;
+                bv = g < ng ? __ldg(reinterpret_cast<const uint32_t*>(a.b + at)) : 0;
+            } else {
+                sv = g < ng ? __ldg(a.s + at) : 0;
+                bv = g < ng ? __ldg(a.b + at) : 0;
+                if (GW == 2 && g + 1 < ng) {
+                    sv |= (uint32_t)__ldg(a.s + at + 1) << 16;
+                    bv |= (uint32_t)__ldg(a.b + at + 1) << 16;
+                }
+            }
+            lj += 2;
+        };
+        fetch();
         for (int n = warp >> 3; n < total; n += 2) {
             if (!all(&b_full[st], ph)) break;
             uint4 w[4];
@@ -387,6 +410,10 @@ __global__ void __launch_bounds__(kThreads, 1) qmm4_tc_kernel(const __grid_const
                 }
                 tmem_st16(to + ua * (kCols / 2) + 16 * i, v);
             }
+            uint32_t* sb = s_sb + ((n & (kScaleRing - 1)) * GPB + kp * GW) * kRows + r;
+            sb[0] = __byte_perm(sv, bv, 0x5410);
+            if (GW == 2) sb[kRows] = __byte_perm(sv, bv, 0x7632);
+            fetch();
             tmem_st_wait();  // (so the codes have arrived, too)
             tc_before_sync();
             __syncwarp();
@@ -406,43 +433,8 @@ __global__ void __launch_bounds__(kThreads, 1) qmm4_tc_kernel(const __grid_const
     } else {
         // ---- sums: a row a lane, half of the tokens a warp --------------------------------
         const int q = warp & 3, half = (warp - kEpiWarp) >> 2, r = 32 * q + lane;
-        const int ng = a.K / GS;
         const uint32_t lanes = tmem + tmem_lane_base(warp) + DCOL + half * NH;
         const float* sums = s_sum + half * NH;
-        // scales and biases of this row's next batches
-        constexpr int kAhead = 3;
-        uint32_t sb[kAhead][2][GPB / 2];
-        int lt = cl, lj = 0;
-        const uint16_t *ps = nullptr, *pb = nullptr;
-        auto rows = [&]() {
-            const long long at = (long long)min(lt * kRows + r, a.N - 1) * ng + b0 * GPB;
-            ps = a.s + at;
-            pb = a.b + at;
-        };
-        rows();
-        auto fetch = [&](uint32_t (&o)[2][GPB / 2]) {
-            if (lt >= a.tiles) return;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint16_t* p = (k ? pb : ps) + lj * GPB;
-                if (a.svec) {  // (then a batch's groups are all there, and aligned)
-                    if (GPB == 4) *reinterpret_cast<uint2*>(o[k]) = __ldg(reinterpret_cast<const uint2*>(p));
-                    else o[k][0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-                } else {
-                    const int left = ng - (b0 + lj) * GPB;
-#pragma unroll
-                    for (int i = 0; i < GPB / 2; ++i)
-                        o[k][i] = (2 * i < left ? __ldg(p + 2 * i) : 0) | ((uint32_t)(2 * i + 1 < left ? __ldg(p + 2 * i + 1) : 0) << 16);
-                }
-            }
-            if (++lj == nb) {
-                lj = 0;
-                lt += ncl;
-                if (lt < a.tiles) rows();
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) fetch(sb[i]);
         bool ok = true;
         int n = 0, it = 0;
         uint64_t acc[NH / 2];  // pairs of tokens
@@ -453,23 +445,14 @@ __global__ void __launch_bounds__(kThreads, 1) qmm4_tc_kernel(const __grid_const
                 const int u = n & 1;
                 ok = ok && all(&b_m[u], (n >> 1) & 1);
                 tc_after_sync();
-                uint32_t now[2][GPB / 2];
+                uint32_t sb[GPB];
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int i = 0; i < GPB / 2; ++i) now[k][i] = sb[0][k][i];
-#pragma unroll
-                for (int i = 0; i + 1 < kAhead; ++i)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int e = 0; e < GPB / 2; ++e) sb[i][k][e] = sb[i + 1][k][e];
-                fetch(sb[kAhead - 1]);
+                for (int g = 0; g < GPB; ++g) sb[g] = s_sb[((n & (kScaleRing - 1)) * GPB + g) * kRows + r];
 #pragma unroll
                 for (int g = 0; g < GPB; ++g) {
                     uint32_t d[NH];
                     tmem_ld_nowait(lanes + u * DSTEP + g * NT, d);
-                    const float s = half_of<DT>(now[0][g / 2], g & 1), b = half_of<DT>(now[1][g / 2], g & 1);
+                    const float s = half_of<DT>(sb[g], 0), b = half_of<DT>(sb[g], 1);
                     const float* xs = sums + (j * GPB + g) * NT;
                     const uint64_t s2 = pair(s, s), b2 = pair(b, b);
                     tmem_ld_wait();
@@ -566,7 +549,7 @@ struct Kernel {
 
 // Shared memory of a block that holds `cap` batches of x, in a cluster of S.
 size_t bytes_of(int cap, int nt, int gs, int S, int stages) {
-    return 1024 + (size_t)stages * kStage + (size_t)cap * (kCols / 64 * nt * 128 + kCols / gs * nt * 4) + (S > 1 ? (size_t)2 * kRows * (nt + 4) * 4 : 0);
+    return 1024 + (size_t)stages * kStage + (size_t)cap * (kCols / 64 * nt * 128 + kCols / gs * nt * 4) + (size_t)kScaleRing * (kCols / gs) * kRows * 4 + (S > 1 ? (size_t)2 * kRows * (nt + 4) * 4 : 0);
 }
 struct Plan {
     int S = 0, cap = 0, stages = 0, clusters = 0;
@@ -639,7 +622,6 @@ int qmm4_tc_launch(const Qmm4Call& c, momij_stream_t st) {
     if (enc(&a.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint32_t*>(c.w), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return MOMIJ_ERR_CUDA;
-    const int ng = c.K / c.gs, gpb = kCols / c.gs;
     a.s = c.s;
     a.b = c.b;
     a.stop = host_stop_flag();
@@ -648,7 +630,7 @@ int qmm4_tc_launch(const Qmm4Call& c, momij_stream_t st) {
     a.N = c.N;
     a.K = c.K;
     a.xvec = host_aligned(c.x, 16) && c.ldx % 8 == 0;
-    a.svec = ng % gpb == 0 && host_aligned(c.s, 2 * gpb) && host_aligned(c.b, 2 * gpb);
+    a.svec = c.K / c.gs % 2 == 0 && host_aligned(c.s, 4) && host_aligned(c.b, 4);
     a.spin = host_spin_limit();
     a.tiles = (c.N + kRows - 1) / kRows;
     a.nbatch = (c.K + kCols - 1) / kCols;

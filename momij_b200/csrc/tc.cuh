@@ -42,6 +42,13 @@ __device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&v)[1
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// Values that a wait has made valid: nothing that uses them moves before this.
+template <int N>
+__device__ __forceinline__ void settle(uint32_t (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
+}
+
 // ---- tcgen05 MMA -------------------------------------------------------------
 // Shared-memory matrix descriptor, K-major, no swizzle: 8-row x 16-byte core
 // matrices; lbo = byte distance of core matrices adjacent along K, sbo = along
