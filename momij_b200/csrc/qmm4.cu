@@ -24,7 +24,8 @@
 // codes and the scales and biases, which a warp copies asynchronously into a ring
 // of its own in shared memory, three batches ahead.  (With the batch after the
 // present one in registers instead: 50 us for 151,936 x 2,048 and one token; the
-// registers left room for 24 warps with 3 KB each in flight.)
+// registers left room for 24 warps with 3 KB each in flight.)  That size takes 36 us,
+// 4.9 TB/s.
 #include <algorithm>
 
 #include "qmm4.cuh"
@@ -359,7 +360,7 @@ extern "C" int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const
                (size_t)2 * warps * cols(mt) * 17 * 4 + 4 * kMaxTok;
     };
     constexpr size_t kBudget = 224 * 1024;
-    // Warps per block (one block an SM) and warps that share a row tile.  Sixteen
+    // Warps per block and warps that share a row tile.  Sixteen
     // warps keep the copies going where their rings leave room for the tokens;
     // eight where they do not, or where sixteen would leave SMs without a round.
     // A tile is shared by the fewest warps (1, 2, 4, 8, at most one a batch) that
@@ -372,6 +373,16 @@ extern "C" int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const
         return k;
     };
     if ((long long)ntiles * share(16) <= 16LL * sms / 2 || bytes(std::min(M, 8), 16) > kBudget) warps = 8;
+    // One token against a matrix of four batches a warp or more: two blocks of eight warps
+    // an SM, which start and end their rounds apart (us for one block / two: 151,936 x
+    // 2,048 34.6 / 33.4, 60,000 x 2,048 19.2 / 17.1, 20,000 x 2,048 8.5 / 7.9; with 3.5
+    // batches, 8,192 x 4,096, 7.3 / 7.7; with seven tokens, whose x each block turns into
+    // an operand, 41.2 / 43.4).
+    int per_sm = 1;
+    if (M == 1 && warps == kMaxWarps && (long long)ntiles * nbatch >= 4LL * kMaxWarps * sms && bytes(1, 8) <= kBudget / 2 - 2048) {
+        warps = 8;
+        per_sm = 2;
+    }
     // tokens per pass: up to 32, fewer where their operand would not fit
     int mt = std::min(M, kMaxTok);
     while (mt > 1 && bytes(mt, warps) > kBudget) --mt;
@@ -388,7 +399,7 @@ extern "C" int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const
     a.wk = share(warps);
     const int wr = warps / a.wk, nround = (ntiles + wr - 1) / wr;
     if (passes > 65535) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
-    const dim3 grid(std::min(nround, sms), passes);
+    const dim3 grid(std::min(nround, per_sm * sms), passes);
     return dtype == MOMIJ_DTYPE_BF16 ? launch_dt<MOMIJ_DTYPE_BF16>(a, grid, warps, smem, nt, gs, vec, stream)
                                      : launch_dt<MOMIJ_DTYPE_F16>(a, grid, warps, smem, nt, gs, vec, stream);
 }
