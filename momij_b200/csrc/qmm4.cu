@@ -359,7 +359,7 @@ extern "C" int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const
         return (size_t)warps * kStages * kStage + (size_t)mt * a.pitch + (size_t)ng * cols(mt) * 4 +
                (size_t)2 * warps * cols(mt) * 17 * 4 + 4 * kMaxTok;
     };
-    constexpr size_t kBudget = 224 * 1024;
+    constexpr size_t kSmemMost = 224 * 1024;
     // Warps per block and warps that share a row tile.  Sixteen
     // warps keep the copies going where their rings leave room for the tokens;
     // eight where they do not, or where sixteen would leave SMs without a round.
@@ -372,21 +372,21 @@ extern "C" int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const
         while (k < 8 && 2 * k <= nbatch && (long long)ntiles * k < 8LL * sms * w) k *= 2;
         return k;
     };
-    if ((long long)ntiles * share(16) <= 16LL * sms / 2 || bytes(std::min(M, 8), 16) > kBudget) warps = 8;
+    if ((long long)ntiles * share(16) <= 16LL * sms / 2 || bytes(std::min(M, 8), 16) > kSmemMost) warps = 8;
     // One token against a matrix of four batches a warp or more: two blocks of eight warps
     // an SM, which start and end their rounds apart (us for one block / two: 151,936 x
     // 2,048 34.6 / 33.4, 60,000 x 2,048 19.2 / 17.1, 20,000 x 2,048 8.5 / 7.9; with 3.5
     // batches, 8,192 x 4,096, 7.3 / 7.7; with seven tokens, whose x each block turns into
     // an operand, 41.2 / 43.4).
     int per_sm = 1;
-    if (M == 1 && warps == kMaxWarps && (long long)ntiles * nbatch >= 4LL * kMaxWarps * sms && bytes(1, 8) <= kBudget / 2 - 2048) {
+    if (M == 1 && warps == kMaxWarps && (long long)ntiles * nbatch >= 4LL * kMaxWarps * sms && bytes(1, 8) <= kSmemMost / 2 - 2048) {
         warps = 8;
         per_sm = 2;
     }
     // tokens per pass: up to 32, fewer where their operand would not fit
     int mt = std::min(M, kMaxTok);
-    while (mt > 1 && bytes(mt, warps) > kBudget) --mt;
-    if (bytes(mt, warps) > kBudget) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
+    while (mt > 1 && bytes(mt, warps) > kSmemMost) --mt;
+    if (bytes(mt, warps) > kSmemMost) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     const int passes = (M + mt - 1) / mt;
     mt = (M + passes - 1) / passes;
     a.mt = mt;

@@ -43,7 +43,7 @@ constexpr int kEpiWarp = kConv, kMmaWarp = kConv + kEpi, kTmaWarp = kMmaWarp + 1
 constexpr int kThreads = 32 * (kFinWarp + kFin);
 constexpr int kMaxStages = 6, kMinStages = 3;
 constexpr int kScaleRing = 8;  // batches: a row's scales are written when the sums of five batches ago are through
-constexpr size_t kBudget = 224 * 1024;
+constexpr size_t kSmemMost = 224 * 1024;
 
 struct TcArgs {
     CUtensorMap map;
@@ -515,7 +515,7 @@ struct Kernel {
         int n = __atomic_load_n(&known[dev], __ATOMIC_ACQUIRE);
         if (n > 0) return n;
         static int granted[64];
-        if (!host_allow_smem(qmm4_tc_kernel<DT, NT, GS, S>, kBudget, granted)) return 0;
+        if (!host_allow_smem(qmm4_tc_kernel<DT, NT, GS, S>, kSmemMost, granted)) return 0;
         cudaLaunchAttribute attr[2];
         cudaLaunchConfig_t cfg = config(8 * S, smem, nullptr, attr);
         if (cudaOccupancyMaxActiveClusters(&n, qmm4_tc_kernel<DT, NT, GS, S>, &cfg) != cudaSuccess) {
@@ -559,14 +559,14 @@ struct Plan {
 template <int DT, int NT, int GS, int S>
 void consider(int tiles, int nbatch, Plan& best, float& least) {
     const int cap = (nbatch + S - 1) / S;
-    if (S > nbatch || bytes_of(cap, NT, GS, S, kMinStages) > kBudget) return;
-    const int n = std::min(Kernel<DT, NT, GS, S>::clusters(kBudget), tiles);
+    if (S > nbatch || bytes_of(cap, NT, GS, S, kMinStages) > kSmemMost) return;
+    const int n = std::min(Kernel<DT, NT, GS, S>::clusters(kSmemMost), tiles);
     if (n < 1) return;
     const float cost = (tiles + n - 1) / n * (cap + (S > 1 ? 1.f : 0.25f)) + cap * (NT / 32.f);
     if (best.S && cost >= least) return;
     least = cost;
     best = Plan{S, cap, kMinStages, n};
-    while (best.stages < kMaxStages && bytes_of(cap, NT, GS, S, best.stages + 1) <= kBudget) ++best.stages;
+    while (best.stages < kMaxStages && bytes_of(cap, NT, GS, S, best.stages + 1) <= kSmemMost) ++best.stages;
 }
 template <int DT, int NT, int GS>
 int run(const Qmm4Call& c, TcArgs& a, momij_stream_t st) {
@@ -595,8 +595,8 @@ int run_dt(const Qmm4Call& c, TcArgs& a, momij_stream_t st) {
 }
 int tokens_per_pass(const Qmm4Call& c) {
     const int nbatch = (c.K + kCols - 1) / kCols, cap = (nbatch + 7) / 8;
-    auto fits = [&](int nt) { return bytes_of(cap, nt, c.gs, 8, kMinStages) <= kBudget && nbatch >= 8; };
-    auto alone = [&](int nt) { return bytes_of(nbatch, nt, c.gs, 1, kMinStages) <= kBudget; };
+    auto fits = [&](int nt) { return bytes_of(cap, nt, c.gs, 8, kMinStages) <= kSmemMost && nbatch >= 8; };
+    auto alone = [&](int nt) { return bytes_of(nbatch, nt, c.gs, 1, kMinStages) <= kSmemMost; };
     const int most = fits(32) || alone(32) ? 32 : fits(16) || alone(16) ? 16 : 0;
     if (!most) return 0;
     const int passes = (c.M + most - 1) / most;
