@@ -21,6 +21,14 @@ __device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// Two results rounded to the activations' type, in one word.
+template <int DT>
+__device__ __forceinline__ uint32_t rounded2(float lo, float hi) {
+    if (DT == MOMIJ_DTYPE_F16) return f16x2_of(lo, hi);
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 // The two 16-bit values of a word as floats.
 template <int DT>
 __device__ __forceinline__ float half_of(uint32_t w, int hi) {

@@ -19,13 +19,13 @@
 // What bounds it: the eight summing warps (a chain of accumulator reads, group sums and
 // scales a batch) and close behind them the conversion (16 KB of codes and their scales
 // cost 16 x 120 instructions); a batch's bytes would come in 750 cycles.  The tensor
-// pipe is busy a tenth of the time.  151,936 x 2,048: 9 tokens 45 us, 32 tokens 58 us
+// pipe is busy a tenth of the time.  151,936 x 2,048: 9 tokens 45 us, 32 tokens 54 us
 // (155 with the other kernel), 26 for the bytes alone; 20,000 x 6,400: 29 and 37 (49
 // and 152).
 // What brought it there: partial sums sent asynchronously and finished by warps of their
 // own (79 us; a releasing arrival per warp costs a microsecond a tile), two sets of
 // converting warps that take batches in turn (51.6), packed sums, scales fetched by the
-// converting warps (47; 63 for 32 tokens).
+// converting warps (47; 63 for 32 tokens), results rounded two at a time (58 for 32).
 #include <algorithm>
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -343,9 +343,10 @@ __global__ void __launch_bounds__(kThreads, 1) qmm4_tc_kernel(const __grid_const
                     const float4 x = *reinterpret_cast<const float4*>(p + k * SLOT + row * PITCH + m);
                     v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
                 }
+                const uint32_t h[2] = {rounded2<DT>(got ? v[0] : NAN, got ? v[1] : NAN), rounded2<DT>(got ? v[2] : NAN, got ? v[3] : NAN)};
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (m + i < a.mt && out < a.N) a.y[(m + i) * a.ldy + out] = Half<DT>::from_f(got ? v[i] : NAN);
+                    if (m + i < a.mt && out < a.N) a.y[(m + i) * a.ldy + out] = (uint16_t)(i & 1 ? h[i / 2] >> 16 : h[i / 2]);
             }
             bar_sync(1, 32 * kFin);  // read: the room is free
             if (ft == 0) mbar_expect_tx(&b_part[u], PART);
@@ -481,9 +482,12 @@ __global__ void __launch_bounds__(kThreads, 1) qmm4_tc_kernel(const __grid_const
             if (S == 1) {
                 const int row = t * kRows + r, most = row < a.N ? a.mt - half * NH : 0;
                 uint16_t* y = a.y + half * NH * a.ldy + row;
+                uint32_t h[NH / 2];
+#pragma unroll
+                for (int i = 0; i < NH / 2; ++i) h[i] = rounded2<DT>(half_pair(acc[i], 0), half_pair(acc[i], 1));
 #pragma unroll
                 for (int i = 0; i < NH; ++i) {
-                    if (i < most) *y = Half<DT>::from_f(half_pair(acc[i / 2], i & 1));
+                    if (i < most) *y = (uint16_t)(i & 1 ? h[i / 2] >> 16 : h[i / 2]);
                     y += a.ldy;
                 }
             } else {
