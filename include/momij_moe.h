@@ -82,6 +82,12 @@ int momij_device_sm_count(void);
  * gqmm2 / router kernel (SeedlessMetal.swift:60, 69-70, 2185, 2730). */
 int momij_set_stop_flag(const int32_t* device_flag);
 
+/* For testing what a flag raised in the middle of a launch leaves behind: block i
+ * of the kernels of momij_qk_norm_rope_append, momij_cache_read and
+ * momij_attention reads word i * words of the stop flag (0, the default: all read
+ * the same word).  Process-wide; applies to calls enqueued afterwards. */
+int momij_set_stop_step(int words);
+
 /* Bound of the device-side waits (polls of an mbarrier or of the grid
  * barrier) before a kernel gives up with MOMIJ_ERR_TIMEOUT: 0 restores the
  * default (about a second), -1 makes every wait give up at once (for testing
@@ -267,7 +273,11 @@ int momij_moe_block(void* h, const void* norm_w, float eps, const void* w_gate, 
  * tokens in qkv / q, or NULL for T / B each; max_q: the most of them in one
  * sequence (0: unknown, up to T).  lens, cu_q and block_table are read on the
  * device; a page, length or row outside its range is skipped and reported as
- * MOMIJ_ERR_PAGE by momij_moe_synchronize(stream, workspace).  D is 64 or 128,
+ * MOMIJ_ERR_PAGE by momij_moe_synchronize(stream, workspace).  The stop flag is
+ * read by each block: one that is raised while a launch starts leaves out what the
+ * blocks that saw it would have written, and is reported as MOMIJ_ERR_STOPPED in
+ * any case (momij_qmm4 and momij_process_logits, which have no workspace, do not
+ * report it).  D is 64 or 128,
  * Hq a multiple of Hkv.  Codes, the rotation table, norm weights and rows of qkv, q_out,
  * k_out and v_out start on 16-byte boundaries, attention's out rows on 8-byte
  * boundaries (its q: any).

@@ -194,6 +194,7 @@ constexpr int kNotApplicable = -1;
 // 60, 69-70) and the bound of the kernels' device-side waits.
 std::atomic<const int32_t*> g_stop_flag{nullptr};
 std::atomic<int> g_spin_limit{0};
+std::atomic<int> g_stop_step{0};
 constexpr int kDefaultSpinLimit = 1 << 22;
 int spin_limit() {
     const int v = g_spin_limit.load();
@@ -1162,6 +1163,7 @@ int host_check_device() { return check_device(); }
 int host_sm_count() { return current_device_sm_count(); }
 bool host_pdl() { return pdl_enabled(); }
 const int32_t* host_stop_flag() { return g_stop_flag.load(); }
+int host_stop_step() { return g_stop_step.load(); }
 int host_spin_limit() { return spin_limit(); }
 void* host_tensor_map_encoder() { return reinterpret_cast<void*>(tensor_map_encoder()); }
 }  // namespace momij
@@ -1239,6 +1241,12 @@ int momij_set_stop_flag(const int32_t* device_flag) {
     return MOMIJ_OK;
 }
 
+int momij_set_stop_step(int words) {
+    if (words < 0) return MOMIJ_ERR_INVALID_ARGUMENT;
+    g_stop_step.store(words);
+    return MOMIJ_OK;
+}
+
 int momij_set_spin_limit(int polls) {
     if (polls < -1) return MOMIJ_ERR_INVALID_ARGUMENT;
     g_spin_limit.store(polls);
@@ -1251,13 +1259,14 @@ int momij_moe_synchronize(momij_stream_t stream, const void* workspace) {
     int32_t hdr[3] = {0, 0, 0};
     if (cudaMemcpy(hdr, workspace, sizeof(hdr), cudaMemcpyDeviceToHost) != cudaSuccess)
         return MOMIJ_ERR_CUDA;
-    if (hdr[1] != MOMIJ_OK) return hdr[1];
-    if (hdr[2] != MOMIJ_OK) {
-        // the error word is sticky on the device; report it once
+    // the error word is sticky on the device; what it holds is reported once,
+    // also where the latest call's own word says the same
+    const int rc = hdr[1] != MOMIJ_OK ? hdr[1] : hdr[2];
+    if (rc != MOMIJ_OK && hdr[2] == rc) {
         int32_t* err = static_cast<int32_t*>(const_cast<void*>(workspace)) + 2;
         if (cudaMemset(err, 0, sizeof(int32_t)) != cudaSuccess) return MOMIJ_ERR_CUDA;
     }
-    return hdr[2];
+    return rc;
 }
 
 int momij_moe_route(const float* logits, int M, int E, int K, int32_t* inds, float* scores,

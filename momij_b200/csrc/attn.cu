@@ -104,9 +104,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     pdl_wait();
-    const int stopped = __syncthreads_or(tid == 0 && a.stop && __ldcg(a.stop) != 0);
-    if (tid == 0 && blockIdx.x == 0) a.ws[kAttnStatus] = stopped ? MOMIJ_ERR_STOPPED : MOMIJ_OK;
-    if (stopped) return;
+    // (a block that saw the stop flag still counts where others wait for its part)
+    const int stopped = __syncthreads_or(tid == 0 && cache_stopped(a.ws, a.stop, a.stop_step));
 
     // ---- prefix sums of the segments' pages, and the segments that have any ---
     const int nseg = a.nb * a.nrb, per = (nseg + kThreads - 1) / kThreads;
@@ -151,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
     if (tid == 0) s_pref[0] = 0;
     __syncthreads();
     // rows that see no key at all
-    if (nfull < nseg)
+    if (nfull < nseg && !stopped)
         for (int sg = blockIdx.x; sg < nseg; sg += gridDim.x)
             if (s_pref[sg + 1] == s_pref[sg]) {
                 const AttnSeq s = attn_sequence(a, a.b0 + sg / a.nrb);
@@ -180,6 +179,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
         const int h = (u - sbase) / np;
         const int hb = sbase + h * np;  // first unit of this (segment, head)
         const int pa = u - hb, pb = min(np, u1 - hb);
+        if (stopped) {
+            if (tid == 0 && pb - pa < np) {
+                int cf, cl, slot;
+                line.sharers(seg, h, hb, np, cf, cl, slot);
+                arrive(a.counters, cf, cl, true);
+            }
+            u = hb + pb;
+            continue;
+        }
 
         // ---- this warp's half pages -------------------------------------------
         const int n_items = 2 * (pb - pa);
@@ -495,10 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                unsigned* ctr = a.counters + cf;
-                const unsigned old = atomicAdd(ctr, 1u);
-                s_last = old == (unsigned)(cl - cf);
-                if (s_last) *ctr = 0u;
+                s_last = arrive(a.counters, cf, cl, false);
                 __threadfence();
             }
             __syncthreads();
@@ -625,6 +630,7 @@ extern "C" int momij_attention(const void* q, long long ldq, void* out, long lon
     a.counters = reinterpret_cast<unsigned*>(ws + kAttnHeader);
     a.parts = reinterpret_cast<float*>(ws + kAttnHeader + kCounterBytes);
     a.stop = host_stop_flag();
+    a.stop_step = host_stop_step();
     a.ldq = ldq;
     a.ldo = ldo;
     a.T = T;

@@ -15,6 +15,7 @@ struct AttnArgs {
     unsigned* counters;  // one per block, zero between calls
     float* parts;        // partial results of segments that several blocks share
     const int32_t* stop;
+    int stop_step;       // words between the blocks' views of the stop flag
     long long ldq, ldo;
     int T, B, Hq, Hkv, G, n_pages, table_cols, window, longest;
     int b0, nb, nrb;     // sequences of this launch, row blocks per sequence
@@ -22,6 +23,18 @@ struct AttnArgs {
     int spin;
     float scale_log2;    // softmax scale * log2(e)
 };
+
+// A block's arrival at the counter of a (segment, head) that the blocks cf .. cl
+// share; one that left its part out (the stop flag, a wait that gave up) counts as
+// well, so that the counter is back at zero after every call.  True for the last
+// arrival if every part is there to be joined.
+constexpr unsigned kLeftOut = 1u << 16;  // (blocks that share: at most 1,024)
+__device__ __forceinline__ bool arrive(unsigned* counter, int cf, int cl, bool left_out) {
+    const unsigned old = atomicAdd(counter + cf, left_out ? 1u + kLeftOut : 1u);
+    if ((old & (kLeftOut - 1u)) != (unsigned)(cl - cf)) return false;
+    counter[cf] = 0u;
+    return !left_out && old < kLeftOut;
+}
 
 struct AttnSeq {
     int past, n, t0, len;

@@ -106,7 +106,7 @@ __device__ __forceinline__ Piece piece_at(const AttnArgs& a, const int* pref, in
     return p;
 }
 
-// Floats of a partial result: O [128][D], maxima, sums.
+// Floats of a partial result: O [128][D], maxima (NaN: the row was left out), sums.
 __host__ __device__ constexpr int part_floats(int D) { return kTileQ * (D + 2); }
 
 __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr) {  // K-major, 128-byte swizzle, 8-row groups 1024 B apart
@@ -310,18 +310,19 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const PrefillArgs pa, in
     const Piece p = piece_at(a, s_pref, start, start + tiles, seg);
     if (r0 >= p.span.rows) return;
     pdl_wait();
-    if (__syncthreads_or(threadIdx.x == 0 && a.stop && __ldcg(a.stop) != 0)) return;
     const float* p0 = a.parts + (long long)slot * part_floats(D);
     const float* p1 = a.parts + (long long)(2 * cf + 2) * part_floats(D);  // of block cf + 1, then every second slot
     auto part = [&](int k) { return k == 0 ? p0 : p1 + (long long)(2 * (k - 1)) * part_floats(D); };
     constexpr int E = D / 32;  // columns a lane
     for (int r = r0 + (threadIdx.x >> 5); r < min(r0 + stretch, p.span.rows); r += 8) {
         float top = -INFINITY, sum = 0.f, o[E] = {};
+        bool left_out = false;
         for (int k0 = 0; k0 <= cl - cf; k0 += 32) {
             // maxima and sums of 32 parts, one a lane
             const bool in = k0 + lane <= cl - cf;
             const float mk = in ? __ldcg(part(k0 + lane) + kTileQ * D + r) : -INFINITY;
             const float lk = in ? __ldcg(part(k0 + lane) + kTileQ * (D + 1) + r) : 0.f;
+            left_out |= mk != mk;
             float nt = mk;
 #pragma unroll
             for (int s = 16; s > 0; s >>= 1) nt = fmaxf(nt, __shfl_xor_sync(0xffffffffu, nt, s));
@@ -343,6 +344,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const PrefillArgs pa, in
                 for (int i = 0; i < E; ++i) o[i] += v[i] * fk;
             }
         }
+        if (__any_sync(0xffffffffu, left_out)) continue;  // reported by the block that left it out
         const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
         const int row = p.row0 + r;
         uint16_t* dst = a.out + (p.sq.t0 + row / a.G) * a.ldo + (p.h * a.G + row % a.G) * D + lane * E;
@@ -383,16 +385,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
         s_abort = 0;
     }
     pdl_wait();
-    const int stopped = __syncthreads_or(tid == 0 && a.stop && __ldcg(a.stop) != 0);
-    if (tid == 0 && blockIdx.x == 0) a.ws[kAttnStatus] = stopped ? MOMIJ_ERR_STOPPED : MOMIJ_OK;
-    if (stopped) return;
+    const int stopped = __syncthreads_or(tid == 0 && cache_stopped(a.ws, a.stop, a.stop_step));
 
     int* s_pref = reinterpret_cast<int*>(smem_raw + SM::kBytes);
     const int nseg = a.nb * a.nrb;
     const Line line = make_line<kThreads>(a, s_pref, gridDim.x);
 
     // rows that see no key at all
-    for (int sg = blockIdx.x; sg < nseg; sg += gridDim.x)
+    for (int sg = blockIdx.x; sg < nseg && !stopped; sg += gridDim.x)
         if (s_pref[sg + 1] == s_pref[sg]) {
             const AttnSeq s = attn_sequence(a, a.b0 + sg / a.nrb);
             const Span p = span_of(a, s, sg % a.nrb);
@@ -406,6 +406,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
     int u0, u1, seg;
     line.range(blockIdx.x, nseg, u0, u1, seg);
     if (u0 >= u1) return;
+    if (stopped) {  // its parts are left out, which whoever joins them has to know
+        for (int u = u0; u < u1;) {
+            const Piece p = piece_at(a, s_pref, u, u1, seg);
+            if (p.jb - p.ja < p.span.tiles) {
+                if (pa.defer) {
+                    float* part = a.parts + (long long)(2 * blockIdx.x + (u != u0)) * part_floats(D);
+                    if (tid < p.span.rows) part[kTileQ * D + tid] = NAN;
+                } else if (tid == 0) {
+                    int cf, cl, slot;
+                    line.sharers(seg, p.h, p.start, p.span.tiles, cf, cl, slot);
+                    arrive(a.counters, cf, cl, true);
+                }
+            }
+            u += p.jb - p.ja;
+        }
+        return;
+    }
 
     if (warp == kMmaWarp) tmem_alloc(&s_tmem, 512);
     tc_before_sync();
@@ -756,14 +773,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             ok = __all_sync(0xffffffffu, ok && wait(&b_o, piece & 1));
             tc_after_sync();
             // ---- results: the two kinds of pages joined, half of the columns a thread -----
-            s_m[e][r] = m;
+            s_m[e][r] = ok ? m : NAN;  // (a maximum itself is never NaN)
             s_l[e][r] = l;
             bar_sync(1, 256);
             const float m0 = s_m[0][r], m1 = s_m[1][r];
             m = fmaxf(m0, m1);
             const float w0 = m0 == m ? 1.f : ex2(m0 - m), w1 = m1 == m ? 1.f : ex2(m1 - m);
             l = s_l[0][r] * w0 + s_l[1][r] * w1;
-            const bool whole = p.ja == 0 && p.jb == p.span.tiles, mine = r < rows && ok;
+            const bool whole = p.ja == 0 && p.jb == p.span.tiles, mine = r < rows && m0 == m0 && m1 == m1;
             float* part = a.parts + (long long)(2 * blockIdx.x + (u != u0)) * part_floats(D);
             uint16_t* dst = a.out + (sq.t0 + tok) * a.ldo + hq * D + e * DH;
             const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
@@ -795,8 +812,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
                 }
             }
             if (!whole) {
-                if (mine && e == 0) {
-                    part[kTileQ * D + r] = m;
+                if (r < rows && e == 0) {
+                    part[kTileQ * D + r] = mine ? m : NAN;
                     part[kTileQ * (D + 1) + r] = l;
                 }
                 if (!pa.defer) {
@@ -805,10 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
                     int cf, cl, slot;
                     line.sharers(seg, h, p.start, p.span.tiles, cf, cl, slot);
                     if (tid == 0) {
-                        unsigned* ctr = a.counters + cf;
-                        const unsigned old = atomicAdd(ctr, 1u);
-                        s_last = old == (unsigned)(cl - cf);
-                        if (s_last) *ctr = 0u;
+                        s_last = arrive(a.counters, cf, cl, *abort != 0);
                         __threadfence();
                     }
                     bar_sync(1, 256);

@@ -12,6 +12,7 @@ int host_check_device();             // MOMIJ_OK or MOMIJ_ERR_NO_DEVICE
 int host_sm_count();                 // of the current device, <= 0 on failure
 bool host_pdl();                     // programmatic dependent launch enabled
 const int32_t* host_stop_flag();     // momij_set_stop_flag's pointer
+int host_stop_step();                // momij_set_stop_step's words
 int host_spin_limit();               // momij_set_spin_limit's bound
 void* host_tensor_map_encoder();     // cuTensorMapEncodeTiled, or NULL
 

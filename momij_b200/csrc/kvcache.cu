@@ -72,6 +72,7 @@ struct AppendArgs {
     const int32_t *table, *lens, *cu;
     int32_t* ws;
     const int32_t* stop;
+    int stop_step;
     long long ld;             // elements between token rows of qkv
     int T, B, Hq, Hkv, n_pages, table_cols, rot, rope_rows, kv_blocks, longest, q_heads;
     Div by_hkv, by_touched, by_longest, by_split;  // (split: warps a token's query heads are shared by)
@@ -270,9 +271,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) append_kernel(const Ap
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = lane % L;
     if (tid == 0) s_top = 0;
     pdl_wait();
-    const int stopped = __syncthreads_or(tid == 0 && a.stop && __ldcg(a.stop) != 0);
-    if (tid == 0 && blockIdx.x == 0 && a.ws) a.ws[kAttnStatus] = stopped ? MOMIJ_ERR_STOPPED : MOMIJ_OK;
-    if (stopped) return;
+    if (__syncthreads_or(tid == 0 && cache_stopped(a.ws, a.stop, a.stop_step))) return;
     const int step = a.rot >> 4;
     const int from = (lane & ~(L - 1)) + (l < step ? l + step : l < 2 * step ? l - step : l);
 
@@ -514,6 +513,7 @@ struct ReadArgs {
     uint16_t *ko, *vo;
     int32_t* ws;
     const int32_t* stop;
+    int stop_step;
     int B, Hkv, n_pages, table_cols, count;
     Div by_hkv, by_parts;
 };
@@ -526,9 +526,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
     __shared__ __align__(16) uint32_t s_v[D * kPage / 4];  // as in append_kernel
     const int tid = threadIdx.x;
     pdl_wait();
-    const int stopped = __syncthreads_or(tid == 0 && a.stop && __ldcg(a.stop) != 0);
-    if (tid == 0 && blockIdx.x == 0 && a.ws) a.ws[kAttnStatus] = stopped ? MOMIJ_ERR_STOPPED : MOMIJ_OK;
-    if (stopped) return;
+    if (__syncthreads_or(tid == 0 && cache_stopped(a.ws, a.stop, a.stop_step))) return;
     int h, j;
     const bool is_v = blockIdx.x & 1;
     const int b = a.by_parts(a.by_hkv(blockIdx.x >> 1, h), j);
@@ -648,6 +646,7 @@ extern "C" int momij_qk_norm_rope_append(const void* qkv, long long ld, void* q_
     a.cu = cu_q;
     a.ws = static_cast<int32_t*>(workspace);
     a.stop = host_stop_flag();
+    a.stop_step = host_stop_step();
     a.ld = ld;
     a.T = T;
     a.B = B;
@@ -705,6 +704,7 @@ extern "C" int momij_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, 
     a.vo = static_cast<uint16_t*>(v_out);
     a.ws = static_cast<int32_t*>(workspace);
     a.stop = host_stop_flag();
+    a.stop_step = host_stop_step();
     a.B = B;
     a.Hkv = Hkv;
     a.n_pages = n_pages;

@@ -26,6 +26,16 @@ __device__ __forceinline__ void cache_error(int32_t* ws, int code) {
     if (ws) atomicMax(ws + kAttnError, code);
 }
 
+// Whether this block leaves its work out (by one thread).  The flag may change
+// while the blocks of a launch start: each that saw it raised says so, and block 0
+// also in the word of the latest call.
+__device__ __forceinline__ bool cache_stopped(int32_t* ws, const int32_t* stop, int step) {
+    const bool on = stop && __ldcg(stop + (long long)blockIdx.x * step) != 0;
+    if (ws && blockIdx.x == 0) ws[kAttnStatus] = on ? MOMIJ_ERR_STOPPED : MOMIJ_OK;
+    if (on) cache_error(ws, MOMIJ_ERR_STOPPED);
+    return on;
+}
+
 // Two codes (bytes `sel` of w) as packed fp16 integers -127 .. 127.
 __device__ __forceinline__ uint32_t codes_f16x2(uint32_t w, uint32_t sel) {
     uint32_t h = __byte_perm(w, 0x64646464u, sel), r;

@@ -80,6 +80,7 @@ def _load() -> ctypes.CDLL:
     L.momij_moe_ep_status.argtypes = [vp, vp]
     L.momij_moe_ep_destroy.argtypes = [vp]
     L.momij_set_stop_flag.argtypes = [vp]
+    L.momij_set_stop_step.argtypes = [i]
     L.momij_set_spin_limit.argtypes = [i]
     L.momij_profile_enable.argtypes = [i]
     L.momij_layer_trace.argtypes = [vp, sz]
@@ -151,6 +152,11 @@ def set_stop_flag(flag: torch.Tensor | None) -> None:
     if flag is not None and (flag.dtype != torch.int32 or not flag.is_cuda):
         raise TypeError("the stop flag is a CUDA int32 tensor")
     _check(lib.momij_set_stop_flag(_ptr(flag)), "set_stop_flag")
+
+
+def set_stop_step(words: int) -> None:
+    """For tests: words of the stop flag between the views of a launch's blocks (0: one view)."""
+    _check(lib.momij_set_stop_step(int(words)), "set_stop_step")
 
 
 def set_spin_limit(polls: int) -> None:
