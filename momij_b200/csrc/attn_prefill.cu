@@ -364,6 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
     __shared__ uint64_t b_q, b_kfull[2], b_kempty[2], b_vfull[2], b_vempty[2], b_s[2], b_p[2][2], b_pv, b_o, b_fin;
     __shared__ uint32_t s_tmem;
     __shared__ float s_m[2][kTileQ], s_l[2][kTileQ];  // of even and odd pages, at the end
+    __shared__ uint32_t s_top[2][kTileQ];             // q's largest magnitude in each half of a row (not s_m: the row's other thread may still read that)
     __shared__ int s_abort, s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;  // warps 0-7 softmax, 8-15 convert, 16 mma
 
@@ -659,9 +660,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             uint32_t top = 0;
 #pragma unroll
             for (int k = 0; k < DH / 2; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-            s_m[e][r] = __uint_as_float(top);
+            s_top[e][r] = top;
             bar_sync(1, 256);
-            top = max(top, __float_as_uint(s_m[1 - e][r]));
+            top = max(top, s_top[1 - e][r]);
             const RowScale rs = row_scale(Half<DT>::to_f((uint16_t)top));
             const float f0 = pa.negate ? -rs.up : rs.up;
             const float fac = a.scale_log2 * rs.down * kRawUnit;

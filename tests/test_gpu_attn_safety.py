@@ -107,3 +107,29 @@ def test_waits_that_give_up_leave_nothing_behind(B, n, length, Hq, Hkv, D):
     for _ in range(2):
         assert torch.equal(attn.attention(*args, workspace=ws), ref)
         moe.synchronize(workspace=ws)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("B,n,Hq,Hkv,D,window", [(24, 40, 32, 8, 64, 0), (20, 50, 24, 8, 128, 100), (3, 700, 16, 4, 64, 300)])
+def test_blocks_that_walk_several_pieces(B, n, Hq, Hkv, D, window, dtype):
+    """More (row tile, head)s than SMs, of unequal lengths: a block carries its stages,
+    phases and shared arrays from one piece to the next."""
+    lens = [n + (b * 97) % 400 for b in range(B)]
+    table, pages = R.block_tables(lens, 1)
+    pool = R.random_pool(pages, Hkv, D, 2)
+    q = (torch.randn(B * n, Hq, D, generator=torch.Generator().manual_seed(3)) * 1.5).to(R.TD[dtype])
+    ws = attn.new_workspace(B * n, Hq)
+    args = (q.cuda(), attn.KVCache(*(t.cuda() for t in pool)), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    out = attn.attention(*args, window=window, workspace=ws)
+    moe.synchronize(workspace=ws)
+    rows = torch.arange(0, B * n, 7)  # (every seventh token in 64 bits; the others by repetition)
+    for b in range(B):
+        at = rows[(rows >= b * n) & (rows < (b + 1) * n)]
+        for t in at.tolist():
+            length = lens[b] - n + (t - b * n) + 1
+            ref, mag, big = R.attention(q[t:t + 1], *pool, table[b:b + 1], [length], [0, 1], window)
+            err = (out[t:t + 1].cpu().double() - ref).abs()
+            assert bool((err <= R.attention_bound(ref, mag, big, D, q.dtype)).all()), (b, t)
+    for _ in range(20):
+        assert torch.equal(attn.attention(*args, window=window, workspace=ws), out)
+    moe.synchronize(workspace=ws)
