@@ -108,14 +108,20 @@ def new_workspace(n_tokens: int, n_heads: int, head_dim: int = 128, device=None)
     return torch.zeros(max(workspace_size(n_tokens, n_heads), HEADER_BYTES), dtype=torch.uint8, device=device or "cuda")
 
 
-def _given(stream, *results):
-    """What a call on a stream of the caller's needs: its handle, and results
-    allocated on the current stream held until that stream is done with them."""
-    if isinstance(stream, torch.cuda.Stream):
-        for t in results:
-            t.record_stream(stream)
-        return stream.cuda_stream
-    return None if stream is None else int(stream)
+def _on(stream, call):
+    """``call()`` on a stream of the caller's (None: the current one): what it allocates
+    and fills is ordered with the kernel, and results are held until the stream that
+    was current is done with them, too."""
+    if stream is None:
+        return call()
+    before = torch.cuda.current_stream()
+    if not isinstance(stream, torch.cuda.Stream):  # a handle; 0 is the default stream's
+        stream = torch.cuda.ExternalStream(int(stream)) if int(stream) else torch.cuda.default_stream()
+    with torch.cuda.stream(stream):
+        out = call()
+    for t in out if isinstance(out, tuple) else (out,):
+        t.record_stream(before)
+    return out
 
 
 def qk_norm_rope_append(qkv: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, *, n_heads: int,
@@ -126,10 +132,8 @@ def qk_norm_rope_append(qkv: torch.Tensor, cache: KVCache, block_table: torch.Te
     """Norms queries and keys per head, rotates them by position and appends keys
     and values to the cache (momij_qk_norm_rope_append).  ``qkv`` [T, (Hq + 2 Hkv) D]
     (rows may be strided); returns the queries [T, Hq, D]."""
-    if stream is not None and q_out is None:
-        q_out = torch.empty(qkv.shape[0], n_heads, cache.k.shape[3], dtype=qkv.dtype, device=qkv.device)
-    return _ops.append(qkv, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lens, n_heads, q_weight, k_weight, eps,
-                       rope, interleaved, cu_q, max_q, q_out, workspace, None if stream is None else _given(stream, q_out))
+    return _on(stream, lambda: _ops.append(qkv, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lens, n_heads, q_weight,
+                                           k_weight, eps, rope, interleaved, cu_q, max_q, q_out, workspace))
 
 
 def cache_read(cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, *, count: int, first: torch.Tensor | None = None,
@@ -138,11 +142,8 @@ def cache_read(cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, *,
     [B, count, Hkv, D]; zeros at and past ``lens[b]``."""
     if dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"values are bf16 or fp16, not {dtype}")
-    out = _ops.read(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lens, first, count, dtype == torch.float16,
-                    workspace, None if stream is None else _given(stream))
-    if stream is not None:
-        _given(stream, *out)
-    return out
+    return _on(stream, lambda: _ops.read(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lens, first, count,
+                                         dtype == torch.float16, workspace))
 
 
 def attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, *, scale: float | None = None,
@@ -150,11 +151,9 @@ def attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens: 
               workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Causal attention of the new tokens' queries ``q`` [T, Hq, D] over the cache
     (momij_attention); ``scale`` defaults to D^-1/2, ``window`` 0 means all positions.
-    Token rows of ``q`` and ``out`` may be strided."""
-    if workspace is None:
-        workspace = new_workspace(q.shape[0], q.shape[1], device=q.device)
-        _given(stream, workspace)
-    if stream is not None and out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    return _ops.attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lens, scale, window, cu_q, max_q, out,
-                          workspace, None if stream is None else _given(stream, out))
+    Token rows of ``q`` and ``out`` may be strided.  Without a workspace the call makes
+    one of its own, and nothing reports a page or length out of range."""
+    def call():
+        ws = new_workspace(q.shape[0], q.shape[1], device=q.device) if workspace is None else workspace
+        return _ops.attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lens, scale, window, cu_q, max_q, out, ws)
+    return _on(stream, call)

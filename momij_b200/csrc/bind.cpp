@@ -93,10 +93,8 @@ int on_current(std::initializer_list<const Tensor*> ts) {
             throw ValueErr("tensors must lie on the current CUDA device");
     return cur;
 }
-momij_stream_t stream_of(PyObject* o, int dev) {
-    if (o == Py_None) return c10::cuda::getCurrentCUDAStream(dev).stream();
-    return reinterpret_cast<momij_stream_t>(static_cast<uintptr_t>(integer(o)));
-}
+// Calls go to the current stream, as their outputs' memory does.
+momij_stream_t stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
 const int32_t* ints(const Tensor* t, const char* name, int64_t n) {
     if (!t) return nullptr;
     if (t->scalar_type() != at::kInt) throw TypeErr(std::string(name) + " is int32");
@@ -168,10 +166,10 @@ void check(int rc, const char* where) {
 void count(Py_ssize_t n, Py_ssize_t want) { type(n == want, "wrong number of arguments"); }
 
 // ---- entries ---------------------------------------------------------------------
-// (qkv, k, v, ks, vs, block_table, lens, n_heads, q_weight, k_weight, eps, rope, interleaved, cu_q, max_q, q_out, workspace, stream)
+// (qkv, k, v, ks, vs, block_table, lens, n_heads, q_weight, k_weight, eps, rope, interleaved, cu_q, max_q, q_out, workspace)
 PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        count(n, 18);
+        count(n, 17);
         const Tensor& qkv = need(o[0], "qkv");
         const Cache c = cache_of(o + 1);
         const Tensor &table = need(o[5], "block_table"), &lens = need(o[6], "lens");
@@ -203,16 +201,16 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
                        PyObject_IsTrue(o[12]), c.k->data_ptr<uint8_t>(), c.v->data_ptr<uint8_t>(), c.ks->data_ptr<float>(),
                        c.vs->data_ptr<float>(), c.pages, table_of(table, B), dim32(table.size(1)), ints(&lens, "lens", B),
                        ints(cu, "cu_q", B + 1), dim32(T), dim32(B), int32(o[14], "max_q"), Hq, c.Hkv, c.D, dt, ptr(ws),
-                       ws ? ws->nbytes() : 0, stream_of(o[17], dev)),
+                       ws ? ws->nbytes() : 0, stream_of(dev)),
               "qkNormRopeAppend");
         return THPVariable_Wrap(std::move(q));
     });
 }
 
-// (k, v, ks, vs, block_table, lens, first, count, f16, workspace, stream)
+// (k, v, ks, vs, block_table, lens, first, count, f16, workspace)
 PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        count(n, 11);
+        count(n, 10);
         const Cache c = cache_of(o);
         const Tensor &table = need(o[4], "block_table"), &lens = need(o[5], "lens");
         const Tensor *first = opt(o[6], "first"), *ws = opt(o[9], "workspace");
@@ -225,7 +223,7 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n) {
         check(F.read(c.k->data_ptr<uint8_t>(), c.v->data_ptr<uint8_t>(), c.ks->data_ptr<float>(), c.vs->data_ptr<float>(), c.pages,
                      table_of(table, B), dim32(table.size(1)), ints(&lens, "lens", B), ints(first, "first", B), cnt, k.data_ptr(),
                      v.data_ptr(), dim32(B), c.Hkv, c.D, f16 ? MOMIJ_DTYPE_F16 : MOMIJ_DTYPE_BF16, ptr(ws), ws ? ws->nbytes() : 0,
-                     stream_of(o[10], dev)),
+                     stream_of(dev)),
               "cacheRead");
         PyObject* kp = THPVariable_Wrap(std::move(k));
         PyObject* vp = THPVariable_Wrap(std::move(v));
@@ -238,10 +236,10 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n) {
     });
 }
 
-// (q, k, v, ks, vs, block_table, lens, scale or None, window, cu_q, max_q, out, workspace, stream)
+// (q, k, v, ks, vs, block_table, lens, scale or None, window, cu_q, max_q, out, workspace)
 PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        count(n, 14);
+        count(n, 13);
         const Tensor& q = need(o[0], "q");
         const Cache c = cache_of(o + 1);
         const Tensor &table = need(o[5], "block_table"), &lens = need(o[6], "lens"), &ws = need(o[12], "workspace");
@@ -266,16 +264,16 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
                           c.k->data_ptr<uint8_t>(), c.v->data_ptr<uint8_t>(), c.ks->data_ptr<float>(), c.vs->data_ptr<float>(), c.pages,
                           table_of(table, B), dim32(table.size(1)), ints(&lens, "lens", B), ints(cu, "cu_q", B + 1), dim32(T), dim32(B),
                           int32(o[10], "max_q"), dim32(Hq), c.Hkv, c.D, (float)scale, int32(o[8], "window"), dt, ws.data_ptr(), ws.nbytes(),
-                          stream_of(o[13], dev)),
+                          stream_of(dev)),
               "attention");
         return THPVariable_Wrap(std::move(out));
     });
 }
 
-// (x, w, scales, biases, gs, out, stream)
+// (x, w, scales, biases, gs, out)
 PyObject* qmm4(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        count(n, 7);
+        count(n, 6);
         const Tensor &x = need(o[0], "x"), &w = need(o[1], "w"), &s = need(o[2], "scales"), &b = need(o[3], "biases");
         const Tensor* given = opt(o[5], "out");
         const int dev = on_current({&x, &w, &s, &b, given});
@@ -297,16 +295,16 @@ PyObject* qmm4(PyObject*, PyObject* const* o, Py_ssize_t n) {
             y = empty({M, N}, x.scalar_type(), dev);
         }
         check(F.qmm4(x.data_ptr(), M > 1 ? x.stride(0) : K, static_cast<const uint32_t*>(w.data_ptr()), s.data_ptr(), b.data_ptr(),
-                     y.data_ptr(), M > 1 ? y.stride(0) : N, dim32(M), dim32(K), dim32(N), gs, dt, stream_of(o[6], dev)),
+                     y.data_ptr(), M > 1 ? y.stride(0) : N, dim32(M), dim32(K), dim32(N), gs, dt, stream_of(dev)),
               "qmm4");
         return THPVariable_Wrap(std::move(y));
     });
 }
 
-// (logits, history, cu_history, repetition, presence, frequency, bias_ids, bias, cu_bias, allowed, out, stream)
+// (logits, history, cu_history, repetition, presence, frequency, bias_ids, bias, cu_bias, allowed, out)
 PyObject* logits(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        count(n, 12);
+        count(n, 11);
         const Tensor& l = need(o[0], "logits");
         const Tensor *h = opt(o[1], "history"), *ch = opt(o[2], "cu_history"), *rep = opt(o[3], "repetition"), *pres = opt(o[4], "presence"),
                      *freq = opt(o[5], "frequency"), *bi = opt(o[6], "bias_ids"), *bv = opt(o[7], "bias"), *cb = opt(o[8], "cu_bias"),
@@ -338,7 +336,7 @@ PyObject* logits(PyObject*, PyObject* const* o, Py_ssize_t n) {
                        ints(ch, "cu_history", B + 1), dim32(nh), floats(rep, "repetition", B), floats(pres, "presence", B),
                        floats(freq, "frequency", B), ints(bi, "bias_ids", nb), floats(bv, "bias", nb), ints(cb, "cu_bias", B + 1), dim32(nb),
                        al ? reinterpret_cast<const uint32_t*>(al->const_data_ptr<int32_t>()) : nullptr,
-                       al ? (B > 1 ? al->stride(0) : al->size(1)) : 0, stream_of(o[11], dev)),
+                       al ? (B > 1 ? al->stride(0) : al->size(1)) : 0, stream_of(dev)),
               "processLogits");
         return THPVariable_Wrap(std::move(out));
     });

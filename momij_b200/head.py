@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import torch
 
-from .attn import _given, _ops
+from .attn import _on, _ops
 
 
 def qmm4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, *, gs: int = 64,
@@ -20,9 +20,7 @@ def qmm4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.T
     """``out`` [M, N] = x [M, K] times the transpose of the 4-bit matrix ``w`` int32/uint32
     [N, K/8] (code k of a word at bits 4k .. 4k+3) with ``scales``, ``biases`` [N, K/gs].
     Rows of ``x`` and ``out`` may be strided."""
-    if stream is not None and out is None:
-        out = torch.empty(x.shape[0], w.shape[0], dtype=x.dtype, device=x.device)
-    return _ops.qmm4(x, w, scales, biases, gs, out, None if stream is None else _given(stream, out))
+    return _on(stream, lambda: _ops.qmm4(x, w, scales, biases, gs, out))
 
 
 def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, cu_history: torch.Tensor | None = None,
@@ -34,7 +32,5 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     offsets ``cu_history`` [B+1]), the biases of ``bias_ids`` / ``cu_bias`` and -inf where
     ``allowed`` (int32 [B, ceil(V/32)], bit v%32 of word v//32) has a zero bit.
     ``out`` may be ``logits`` itself where that is fp32."""
-    if stream is not None and out is None:
-        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
-    return _ops.logits(logits, history, cu_history, repetition, presence, frequency, bias_ids, bias, cu_bias, allowed, out,
-                       None if stream is None else _given(stream, out))
+    return _on(stream, lambda: _ops.logits(logits, history, cu_history, repetition, presence, frequency, bias_ids, bias, cu_bias, allowed,
+                                           out))

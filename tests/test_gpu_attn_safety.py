@@ -133,3 +133,40 @@ def test_blocks_that_walk_several_pieces(B, n, Hq, Hkv, D, window, dtype):
     for _ in range(20):
         assert torch.equal(attn.attention(*args, window=window, workspace=ws), out)
     moe.synchronize(workspace=ws)
+
+
+@pytest.mark.parametrize("handle", [False, True])
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_stream_of_the_callers_beside_a_busy_one(n, handle):
+    """The current stream is busy, the call's stream is not: nothing that the call needs
+    (a workspace of its own, filled with zeros) may wait for the busy one, and what it
+    allocates is not memory that the busy one still uses."""
+    from momij_b200 import head
+    args = device_args(2, n, 2000, 8, 2, 64, "bf16")
+    ref = attn.attention(*args)
+    w, s, b = torch.randint(0, 1 << 30, (64, 32), dtype=torch.int32, device="cuda"), *(torch.rand(64, 4, device="cuda").bfloat16() for _ in range(2))
+    x = torch.randn(2, 256, device="cuda").bfloat16()
+    qkv = torch.randn(2 * n, 12 * 64, device="cuda").bfloat16()
+    y, kv = head.qmm4(x, w, s, b), attn.cache_read(*args[1:], count=70)
+    cache = attn.KVCache(*(t.clone() for t in (args[1].k, args[1].v, args[1].k_scale, args[1].v_scale)))
+    q = attn.qk_norm_rope_append(qkv, cache, *args[2:], n_heads=8)
+    logits = torch.randn(2, 500, device="cuda")
+    side = torch.cuda.Stream()
+    given = side.cuda_stream if handle else side
+    size = attn.workspace_size(2 * n, 8)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        busy = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(2)]  # freed memory full of ones
+        busy += [torch.full((ref.numel(),), 1.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        for t in busy:
+            t.fill_(1)  # enqueued behind it, and then freed
+        del t, busy
+        out = attn.attention(*args, stream=given)
+        y2, kv2 = head.qmm4(x, w, s, b, stream=given), attn.cache_read(*args[1:], count=70, stream=given)
+        q2 = attn.qk_norm_rope_append(qkv, cache, *args[2:], n_heads=8, stream=given)
+        l2 = head.process_logits(logits, stream=given)
+        side.synchronize()
+        torch.cuda.synchronize()
+        for a, r in ((out, ref), (y2, y), (kv2[0], kv[0]), (kv2[1], kv[1]), (q2, q), (l2, logits)):
+            assert torch.equal(a, r)
