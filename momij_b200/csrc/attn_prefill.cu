@@ -300,16 +300,17 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const PrefillArgs pa, in
     const int nseg = a.nb * a.nrb, lane = threadIdx.x & 31;
     const Line line = make_line<256>(a, s_pref, grid);
     int seg = blockIdx.x / a.Hkv;
-    const int h = blockIdx.x - seg * a.Hkv, tiles = s_pref[seg + 1] - s_pref[seg];
-    if (seg >= nseg || tiles == 0) return;
+    const int h = blockIdx.x - seg * a.Hkv, tiles = s_pref[seg + 1] - s_pref[seg];  // (the grid has the segments' heads)
     const int start = s_pref[seg] * a.Hkv + h * tiles;
-    int cf, cl, slot;
-    line.sharers(seg, h, start, tiles, cf, cl, slot);
+    int cf = 0, cl = 0, slot = 0;
+    if (tiles > 0) line.sharers(seg, h, start, tiles, cf, cl, slot);
+    // On every path, also with nothing to join: the next kernel's wait covers this grid
+    // alone, which must not be over before the main kernel is.
+    pdl_wait();
     const int r0 = blockIdx.y * stretch;
     if (cl == cf) return;
     const Piece p = piece_at(a, s_pref, start, start + tiles, seg);
     if (r0 >= p.span.rows) return;
-    pdl_wait();
     const float* p0 = a.parts + (long long)slot * part_floats(D);
     const float* p1 = a.parts + (long long)(2 * cf + 2) * part_floats(D);  // of block cf + 1, then every second slot
     auto part = [&](int k) { return k == 0 ? p0 : p1 + (long long)(2 * (k - 1)) * part_floats(D); };

@@ -228,10 +228,11 @@ __global__ void __launch_bounds__(kNameThreads) name_kernel(const Args a) {
     const int stop = tid == 0 && a.stop && __ldcg(a.stop) != 0;
     const Row r = row_of(a, row);
     const long long in0 = row * a.ld + v0, out0 = (long long)row * a.V + v0;
-    if (__syncthreads_or(stop)) return;  // (also publishes the cleared counts)
-    count_ids<kNameThreads>(a, r, v0, nv, s_word);
+    const int stopped = __syncthreads_or(stop);  // (also publishes the cleared counts)
+    if (!stopped) count_ids<kNameThreads>(a, r, v0, nv, s_word);
     __syncthreads();
-    pdl_wait();  // the copy is complete
+    pdl_wait();  // the copy is complete (a stopped block waits too: the next kernel's wait covers this grid alone)
+    if (stopped) return;
     for (int i0 = tid * 4; i0 < nv; i0 += kNameThreads * 16) {
         uint32_t named = 0;
 #pragma unroll

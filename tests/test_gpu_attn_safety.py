@@ -170,3 +170,26 @@ def test_a_stream_of_the_callers_beside_a_busy_one(n, handle):
         torch.cuda.synchronize()
         for a, r in ((out, ref), (y2, y), (kv2[0], kv[0]), (kv2[1], kv[1]), (q2, q), (l2, logits)):
             assert torch.equal(a, r)
+
+
+@pytest.mark.parametrize("length", [30, 400])
+def test_attention_with_nothing_to_join_is_over_before_the_next_operator(length):
+    """Few heads and 17 rows or more bring a joining launch, which a short context leaves
+    nothing to do; what comes next reads the main kernel's results all the same."""
+    from momij_b200 import head
+    q, *rest = device_args(1, 20, length, 4, 1, 64, "bf16")
+    w = torch.randint(-2 ** 31, 2 ** 31, (300, 32), dtype=torch.int64, device="cuda").to(torch.int32)
+    s, b = (torch.rand(300, 4, device="cuda").bfloat16() - 0.5 for _ in range(2))
+    ws, out = attn.new_workspace(20, 4), torch.empty_like(q)
+    wants, gots = [], []
+    qs = [torch.randn_like(q) for _ in range(40)]
+    for x in qs:
+        o = attn.attention(x, *rest, workspace=ws)
+        torch.cuda.synchronize()
+        wants.append(head.qmm4(o.flatten(1), w, s, b))
+    torch.cuda.synchronize()
+    for x in qs:
+        gots.append(head.qmm4(attn.attention(x, *rest, out=out, workspace=ws).flatten(1), w, s, b))
+    moe.synchronize(workspace=ws)
+    for a, r in zip(gots, wants):
+        assert torch.equal(a, r)
