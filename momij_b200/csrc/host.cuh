@@ -5,6 +5,7 @@
 #include <utility>
 
 #include "common.cuh"
+#include "grant.cuh"
 
 namespace momij {
 
@@ -31,13 +32,11 @@ inline bool host_allow_smem(K kern, size_t smem, int (&granted)[64]) {
     if (smem <= 48 * 1024) return true;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
-    if (__atomic_load_n(&granted[dev], __ATOMIC_ACQUIRE) >= (int)smem) return true;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    return grant_at_least(granted[dev], (int)smem, [&](int size) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, size) == cudaSuccess) return true;
         cudaGetLastError();
         return false;
-    }
-    __atomic_store_n(&granted[dev], (int)smem, __ATOMIC_RELEASE);
-    return true;
+    });
 }
 
 // Launch with programmatic dependent launch: the kernel starts while the
