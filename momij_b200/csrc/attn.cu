@@ -640,7 +640,9 @@ extern "C" int momij_attention(const void* q, long long ldq, void* out, long lon
     a.G = Hq / Hkv;
     a.n_pages = n_pages;
     a.table_cols = table_cols;
-    a.window = window;
+    // A window of all the positions that the table has room for sees everything; below
+    // that, positions (from -T on) less the window stay within 32 bits.
+    a.window = window >= (long long)table_cols * kPage ? 0 : window;
     a.longest = cu_q ? (max_q > 0 ? std::min(max_q, T) : T) : T / B;
     a.qvec = host_aligned(q, 16) && ldq % 8 == 0;
     a.spin = host_spin_limit();

@@ -193,3 +193,20 @@ def test_attention_with_nothing_to_join_is_over_before_the_next_operator(length)
     moe.synchronize(workspace=ws)
     for a, r in zip(gots, wants):
         assert torch.equal(a, r)
+
+
+@pytest.mark.parametrize("n", [5, 40])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 30, 512, 511])
+def test_windows_wider_than_the_cache(n, window):
+    """Wider than anything, with caches shorter than the queries (positions below zero)."""
+    lens = [2, 500, 0, n, 130]
+    table, pages = R.block_tables(lens, 6)
+    cache = attn.KVCache(*(t.cuda() for t in R.random_pool(pages, 2, 64, 7)))
+    q = torch.randn(5 * n, 8, 64, generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    ws = attn.new_workspace(5 * n, 8)
+    args = (q, cache, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    assert table.shape[1] * 64 == 512
+    out = [attn.attention(*args, window=w, workspace=ws) for w in (0, window)]
+    moe.synchronize(workspace=ws)
+    assert torch.equal(*out)
+    assert (out[0][:n - 2] == 0).all() and not (out[0][n - 2:n] == 0).all()
