@@ -80,7 +80,7 @@ struct AppendArgs {
 };
 
 struct Seq {
-    int past, n, t0;  // tokens before the call, tokens added, first row of qkv
+    int len, past, n, t0;  // tokens after and before the call, tokens added, first row of qkv
 };
 __device__ __forceinline__ Seq sequence(const AppendArgs& a, int b) {
     Seq s;
@@ -91,12 +91,14 @@ __device__ __forceinline__ Seq sequence(const AppendArgs& a, int b) {
         s.n = a.T / a.B;
         s.t0 = b * s.n;
     }
-    s.past = __ldg(a.lens + b) - s.n;
+    s.len = __ldg(a.lens + b);
+    s.past = (int)((unsigned)s.len - (unsigned)s.n);  // (garbage lengths may wrap: usable() goes by len)
     return s;
 }
 // Whether the rows and positions of a sequence are usable at all.
 __device__ __forceinline__ bool usable(const AppendArgs& a, const Seq& s) {
-    return s.n >= 0 && s.n <= a.longest && s.past >= 0 && s.t0 >= 0 && s.n <= a.T - s.t0 && (!a.rope || s.past + s.n <= a.rope_rows);
+    return s.n >= 0 && s.n <= a.longest && s.len >= s.n && s.len <= (long long)a.table_cols * kPage && s.t0 >= 0 &&
+           s.n <= a.T - s.t0 && (!a.rope || s.len <= a.rope_rows);
 }
 
 // Two 16-bit values of a word as floats, and two floats rounded into one.
@@ -621,7 +623,7 @@ extern "C" int momij_qk_norm_rope_append(const void* qkv, long long ld, void* q_
     if (int rc = host_check_device()) return rc;
     if (T < 0 || B < 0 || n_pages < 0 || table_cols < 0 || rope_rows < 0 || max_q < 0) return MOMIJ_ERR_INVALID_ARGUMENT;
     if (dtype != MOMIJ_DTYPE_BF16 && dtype != MOMIJ_DTYPE_F16) return MOMIJ_ERR_INVALID_ARGUMENT;
-    if (Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || (D != 64 && D != 128) || rot < 0 || rot > D || rot % 16 != 0)
+    if (Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || (D != 64 && D != 128) || rot < 0 || rot > D || rot % 16 != 0 || table_cols > (1 << 24))
         return MOMIJ_ERR_UNSUPPORTED_SHAPE;
     if (T == 0 || B == 0) return MOMIJ_OK;
     if (!cu_q && T % B != 0) return MOMIJ_ERR_INVALID_ARGUMENT;

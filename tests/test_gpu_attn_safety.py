@@ -210,3 +210,35 @@ def test_windows_wider_than_the_cache(n, window):
     moe.synchronize(workspace=ws)
     assert torch.equal(*out)
     assert (out[0][:n - 2] == 0).all() and not (out[0][n - 2:n] == 0).all()
+
+
+@pytest.mark.parametrize("n", [1, 3])
+@pytest.mark.parametrize("bad", [-2 ** 31, -2 ** 31 + 1, -1, 257, 2 ** 31 - 1, 2 ** 31 - 64])
+def test_append_skips_and_reports_lengths_out_of_range(n, bad):
+    """With and without a table of angles: lengths that positions computed from them would
+    wrap at are skipped like any other, and the sequence beside them is served."""
+    for rope in (None, attn.rope_table(256, 64)):
+        _, cache, table, lens = device_args(2, 1, 256, 4, 2, 64, "bf16")  # (four columns)
+        x = torch.randn(2 * n, 8 * 64, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+        ws = attn.new_workspace(1, 1)
+        tensors = (cache.k, cache.v, cache.k_scale, cache.v_scale)
+        good = attn.KVCache(*(t.clone() for t in tensors))
+        ref = attn.qk_norm_rope_append(x[:n], good, table[:1], lens[:1], n_heads=4, rope=rope, workspace=ws)
+        moe.synchronize(workspace=ws)
+        lens[1] = bad
+        q = attn.qk_norm_rope_append(x, cache, table, lens, n_heads=4, rope=rope, workspace=ws)
+        with pytest.raises(moe.SeedlessError) as e:
+            moe.synchronize(workspace=ws)
+        assert e.value.status == 11
+        assert torch.equal(q[:n], ref) and all(torch.equal(a, getattr(good, f)) for a, f in zip(tensors, ("k", "v", "k_scale", "v_scale")))
+
+
+def test_tables_wider_than_positions_can_count_are_refused():
+    q, cache, _, lens = device_args(1, 1, 64, 4, 2, 64, "bf16")
+    table = torch.zeros(1, 2 ** 24 + 1, dtype=torch.int32, device="cuda")
+    ws = attn.new_workspace(1, 4)
+    for call in (lambda: attn.attention(q, cache, table, lens, workspace=ws),
+                 lambda: attn.qk_norm_rope_append(torch.zeros(1, 8 * 64, dtype=q.dtype, device="cuda"), cache, table, lens, n_heads=4)):
+        with pytest.raises(moe.SeedlessError) as e:
+            call()
+        assert e.value.status == moe.UNSUPPORTED_SHAPE
