@@ -117,8 +117,9 @@ struct Line {
             seg = s / Hkv;
             const int n = pref[seg + 1] - pref[seg], k = min(parts, n);
             const int at = pref[seg] * Hkv + (s - seg * Hkv) * n;
-            u0 = part < k ? at + n * part / k : at;
-            u1 = part < k ? at + n * (part + 1) / k : at;
+            const int each = n / k, rest = n - each * k;  // (n times a part may pass 32 bits)
+            u0 = part < k ? at + each * part + rest * part / k : at;
+            u1 = part < k ? at + each * (part + 1) + rest * (part + 1) / k : at;
             return;
         }
         u0 = share(block);

@@ -242,3 +242,22 @@ def test_tables_wider_than_positions_can_count_are_refused():
         with pytest.raises(moe.SeedlessError) as e:
             call()
         assert e.value.status == moe.UNSUPPORTED_SHAPE
+
+
+@pytest.mark.parametrize("n", [1, 17])
+def test_the_longest_context(n):
+    """2^30 tokens, all of them one page: with queries of zeros, the mean of its values.
+    Bound: every sum in the order of the tokens, 2^-23 for each of a block's additions
+    (its tiles, or its warps' half pages, and the products' steps of 16 tokens)."""
+    table = torch.zeros(1, 2 ** 24, dtype=torch.int32, device="cuda")
+    pool = R.random_pool(1, 1, 64, 5)
+    cache = attn.KVCache(*(t.cuda() for t in pool))
+    lens = torch.tensor([2 ** 30], dtype=torch.int32, device="cuda")
+    ws = attn.new_workspace(n, 1)
+    out = attn.attention(torch.zeros(n, 1, 64, dtype=torch.bfloat16, device="cuda"), cache, table, lens, workspace=ws)
+    moe.synchronize(workspace=ws)
+    v = R.values(*pool)[1][0, 0]
+    want, mag = v.mean(0), v.abs().mean(0)  # (the last queries miss up to 16 of 2^30 tokens)
+    steps = 2 ** 30 / 16 / moe.lib.momij_device_sm_count()
+    err = (out[:, 0].cpu().double() - want).abs()
+    assert bool((err <= 2 ** -8 * want.abs() + 2 * steps * 2 ** -23 * mag).all()), float((err / mag).max())
