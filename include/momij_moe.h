@@ -278,7 +278,7 @@ int momij_moe_block(void* h, const void* norm_w, float eps, const void* w_gate, 
  * blocks that saw it would have written, and is reported as MOMIJ_ERR_STOPPED in
  * any case (momij_qmm4 and momij_process_logits, which have no workspace, do not
  * report it).  D is 64 or 128,
- * Hq a multiple of Hkv, table_cols at most 2^24.  Codes, the rotation table, norm weights and rows of qkv, q_out,
+ * Hq a multiple of Hkv, table_cols at most 2^24.  Codes, workspaces, the rotation table, norm weights and rows of qkv, q_out,
  * k_out and v_out start on 16-byte boundaries, attention's out rows on 8-byte
  * boundaries (its q: any).
  */

@@ -54,6 +54,12 @@ const Tensor* opt(PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) throw TypeErr(std::string(name) + " is a tensor");
     return &THPVariable_Unpack(o);
 }
+// A workspace's bytes lie together: a strided or expanded tensor has others between, or fewer.
+const Tensor* workspace(PyObject* o) {
+    const Tensor* t = opt(o, "workspace");
+    value(!t || t->is_contiguous(), "a workspace is a contiguous tensor");
+    return t;
+}
 const Tensor& need(PyObject* o, const char* name) {
     const Tensor* t = opt(o, name);
     if (!t) throw TypeErr(std::string(name) + " is a tensor");
@@ -175,7 +181,7 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const Tensor &table = need(o[5], "block_table"), &lens = need(o[6], "lens");
         const int Hq = int32(o[7], "n_heads");
         const Tensor *qw = opt(o[8], "q_weight"), *kw = opt(o[9], "k_weight"), *rope = opt(o[11], "rope"), *cu = opt(o[13], "cu_q"),
-                     *given = opt(o[15], "q_out"), *ws = opt(o[16], "workspace");
+                     *given = opt(o[15], "q_out"), *ws = workspace(o[16]);
         const int dev = on_current({&qkv, c.k, c.v, c.ks, c.vs, &table, &lens, qw, kw, rope, cu, given, ws});
         const int dt = half_code(qkv);
         value(qkv.dim() == 2 && lens.dim() == 1, "qkv is [T, (Hq + 2 Hkv) D] and lens [B]");
@@ -213,7 +219,7 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n) {
         count(n, 10);
         const Cache c = cache_of(o);
         const Tensor &table = need(o[4], "block_table"), &lens = need(o[5], "lens");
-        const Tensor *first = opt(o[6], "first"), *ws = opt(o[9], "workspace");
+        const Tensor *first = opt(o[6], "first"), *ws = workspace(o[9]);
         const int dev = on_current({c.k, c.v, c.ks, c.vs, &table, &lens, first, ws});
         const int cnt = int32(o[7], "count"), f16 = PyObject_IsTrue(o[8]);
         value(lens.dim() == 1 && cnt >= 0, "lens is [B], count not negative");
@@ -242,8 +248,10 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
         count(n, 13);
         const Tensor& q = need(o[0], "q");
         const Cache c = cache_of(o + 1);
-        const Tensor &table = need(o[5], "block_table"), &lens = need(o[6], "lens"), &ws = need(o[12], "workspace");
-        const Tensor *cu = opt(o[9], "cu_q"), *given = opt(o[11], "out");
+        const Tensor &table = need(o[5], "block_table"), &lens = need(o[6], "lens");
+        const Tensor *cu = opt(o[9], "cu_q"), *given = opt(o[11], "out"), *wsp = workspace(o[12]);
+        type(wsp != nullptr, "workspace is a tensor");
+        const Tensor& ws = *wsp;
         const int dev = on_current({&q, c.k, c.v, c.ks, c.vs, &table, &lens, cu, given, &ws});
         const int dt = half_code(q);
         value(q.dim() == 3 && lens.dim() == 1, "q is [T, Hq, D] and lens [B]");

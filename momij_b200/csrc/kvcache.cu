@@ -632,6 +632,7 @@ extern "C" int momij_qk_norm_rope_append(const void* qkv, long long ld, void* q_
     if (ld < (long long)(Hq + 2 * Hkv) * D || ld % 8 != 0 || !host_aligned(qkv, 16) || !host_aligned(q_out, 16) || !host_aligned(rope, 16) ||
         !host_aligned(k_codes, 16) || !host_aligned(v_codes, 16) || !host_aligned(q_weight, 16) || !host_aligned(k_weight, 16))
         return MOMIJ_ERR_INVALID_ARGUMENT;
+    if (!host_aligned(workspace, 16)) return MOMIJ_ERR_INVALID_ARGUMENT;
     if (workspace && workspace_bytes < kAttnHeader) return MOMIJ_ERR_WORKSPACE;
     AppendArgs a{};
     a.qkv = static_cast<const uint16_t*>(qkv);
@@ -693,6 +694,7 @@ extern "C" int momij_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, 
     if (!k_codes || !v_codes || !k_scales || !v_scales || !block_table || !lens || !k_out || !v_out) return MOMIJ_ERR_INVALID_ARGUMENT;
     if (!host_aligned(k_codes, 16) || !host_aligned(v_codes, 16) || !host_aligned(k_out, 16) || !host_aligned(v_out, 16))
         return MOMIJ_ERR_INVALID_ARGUMENT;
+    if (!host_aligned(workspace, 16)) return MOMIJ_ERR_INVALID_ARGUMENT;
     if (workspace && workspace_bytes < kAttnHeader) return MOMIJ_ERR_WORKSPACE;
     ReadArgs a{};
     a.k = k_codes;

@@ -261,3 +261,22 @@ def test_the_longest_context(n):
     steps = 2 ** 30 / 16 / moe.lib.momij_device_sm_count()
     err = (out[:, 0].cpu().double() - want).abs()
     assert bool((err <= 2 ** -8 * want.abs() + 2 * steps * 2 ** -23 * mag).all()), float((err / mag).max())
+
+
+def test_workspaces_that_do_not_lie_where_their_bytes_say_are_refused():
+    q, cache, table, lens = device_args(1, 1, 64, 4, 2, 64, "bf16")
+    x = torch.zeros(1, 8 * 64, dtype=q.dtype, device="cuda")
+    n = attn.workspace_size(1, 4)
+    calls = (lambda ws: attn.attention(q, cache, table, lens, workspace=ws),
+             lambda ws: attn.qk_norm_rope_append(x, cache, table, lens, n_heads=4, workspace=ws),
+             lambda ws: attn.cache_read(cache, table, lens, count=4, workspace=ws))
+    for call in calls:
+        for bad in (torch.zeros(1, dtype=torch.uint8, device="cuda").expand(n), torch.zeros(2 * n, dtype=torch.uint8, device="cuda")[::2]):
+            with pytest.raises(ValueError):
+                call(bad)
+        for off in (1, 2, 4):
+            with pytest.raises(moe.SeedlessError) as e:
+                call(torch.zeros(n + 16, dtype=torch.uint8, device="cuda")[off:off + n])
+            assert e.value.status == moe.INVALID_ARGUMENT
+        call(torch.zeros(n + 16, dtype=torch.uint8, device="cuda")[16:])
+    torch.cuda.synchronize()
