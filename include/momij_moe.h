@@ -266,7 +266,9 @@ int momij_moe_block(void* h, const void* norm_w, float eps, const void* w_gate, 
  *   k_codes uint8 [n_pages, Hkv, 64, D]   v_codes uint8 [n_pages, Hkv, D, 64]
  *   k_scales, v_scales fp32 [n_pages, Hkv]
  * A code c stands for (c - 128) * scale of its page and head (c in 1..255; a
- * scale is 0, NaN or between 2^-64 and 2^100).  block_table int32 [B,
+ * scale is 0, NaN or between 2^-64 and 2^100; the V scales of the pages that a
+ * query sees lie within 2^100 of each other, and below 2^40 where a page of zeros is
+ * among them, or pages of much smaller scales lose their weight).  block_table int32 [B,
  * table_cols]: the page of tokens 64 i .. 64 i + 63 of sequence b.  lens int32
  * [B]: tokens of each sequence in the cache, INCLUDING the ones that a call
  * appends or queries.  cu_q int32 [B + 1]: row offsets of each sequence's new

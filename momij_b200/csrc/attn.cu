@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
                 }
             }
             // weights: x = fac ks (q.c - 128 sum q) + log2 vs; a page of zeros (scale 0) keeps its weight in the sum
-            const float lv = vs == 0.f ? 0.f : __log2f(vs), iv = vs == 0.f ? 1.f : __fdividef(1.f, vs);
+            const float lv = scale_log2_of(vs), iv = scale_inverse_of(vs);
             const bool inside = t0 + 32 <= all_hi && t0 >= all_lo;
             uint32_t p[NB][4];
 #pragma unroll

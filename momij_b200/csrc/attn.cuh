@@ -65,6 +65,14 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// How a page's V scale b enters: log2 b in the exponent of its tokens' weights, 1 / b
+// in their sum.  A page of zeros (scale 0) adds nothing to the outputs but keeps its
+// weight in the sum: as if its scale were the smallest that an append writes, so
+// that no page beside it loses bits to its maximum.
+constexpr float kZeroPageLog2 = -64.f;
+__device__ __forceinline__ float scale_log2_of(float b) { return b == 0.f ? kZeroPageLog2 : __log2f(b); }
+__device__ __forceinline__ float scale_inverse_of(float b) { return b == 0.f ? 0x1p64f : __fdividef(1.f, b); }
+
 // The power of two that brings a row's largest magnitude to 2^13 .. 2^14, and
 // its inverse, from the exponent alone; 1 for zeros, infinities and NaN.  Rows
 // whose largest magnitude is below 2^-113 stay smaller (their scores are nil).

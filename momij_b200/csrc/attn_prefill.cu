@@ -598,8 +598,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             if (ct < 2) {
                 float* o = s_scale[j & (kScaleRing - 1)][ct];
                 o[0] = sc[0];
-                o[1] = sc[1] == 0.f ? 0.f : __log2f(sc[1]);  // a page of zeros keeps its weight in the sum
-                o[2] = sc[1] == 0.f ? 1.f : __fdividef(1.f, sc[1]);
+                o[1] = scale_log2_of(sc[1]);
+                o[2] = scale_inverse_of(sc[1]);
             }
             // K as c * 2^-24; the second page's rows follow the first's 64, 4 KB of codes are 32 or 64 rows
 #pragma unroll

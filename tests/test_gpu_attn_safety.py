@@ -280,3 +280,26 @@ def test_workspaces_that_do_not_lie_where_their_bytes_say_are_refused():
             assert e.value.status == moe.INVALID_ARGUMENT
         call(torch.zeros(n + 16, dtype=torch.uint8, device="cuda")[16:])
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("mult", [2.0 ** -45, 2.0 ** -20, 2.0 ** 30])
+def test_pages_of_zeros_beside_small_and_large_values(mult, n):
+    """Values scaled down or up, two pages of zeros (one of each parity, one of them the
+    first) among them: the others keep their bits, the zeros their weight."""
+    lens, Hkv, D = [400], 2, 64
+    table, pages = R.block_tables(lens, 9)
+    k, v, ks, vs = R.random_pool(pages, Hkv, D, 10)
+    vs *= mult
+    for i in (0, 3):
+        p = int(table[0, i])
+        v[p], vs[p] = 128, 0.0
+    q = torch.randn(n, 8, D, generator=torch.Generator().manual_seed(11)).bfloat16()
+    ws = attn.new_workspace(n, 8)
+    out = attn.attention(q.cuda(), attn.KVCache(k.cuda(), v.cuda(), ks.cuda(), vs.cuda()), table.cuda(),
+                         torch.tensor(lens, dtype=torch.int32).cuda(), workspace=ws)
+    moe.synchronize(workspace=ws)
+    ref, mag, big = R.attention(q, k, v, ks, vs, table, lens, [0, n])
+    bound = R.attention_bound(ref / mult, mag / mult, big, D, q.dtype) * mult  # (its last term is for values near one)
+    err = (out.cpu().double() - ref).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
