@@ -534,10 +534,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
     const int b = a.by_parts(a.by_hkv(blockIdx.x >> 1, h), j);
     const long long from = a.first ? __ldg(a.first + b) : 0;
     const int len = __ldg(a.lens + b);
-    if (from < 0) {
-        if (tid == 0) cache_error(a.ws, MOMIJ_ERR_PAGE);
-        return;
-    }
+    if (tid == 0 && (from < 0 || len < 0 || len > (long long)a.table_cols * kPage)) cache_error(a.ws, MOMIJ_ERR_PAGE);
+    if (from < 0) return;
     const long long blk = from / kPage + j, p0 = blk * kPage;
     const long long t0 = p0 > from ? p0 : from, t1 = p0 + kPage < from + a.count ? p0 + kPage : from + a.count;  // tokens asked for here
     if (t0 >= t1) return;

@@ -303,3 +303,19 @@ def test_pages_of_zeros_beside_small_and_large_values(mult, n):
     bound = R.attention_bound(ref / mult, mag / mult, big, D, q.dtype) * mult  # (its last term is for values near one)
     err = (out.cpu().double() - ref).abs()
     assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("bad", [-1, -2 ** 31, 257, 2 ** 31 - 1])
+def test_cache_read_reports_lengths_out_of_range(bad):
+    _, cache, table, lens = device_args(2, 1, 256, 4, 2, 64, "bf16")  # (four columns)
+    ws = attn.new_workspace(1, 1)
+    want = attn.cache_read(cache, table, lens, count=100, workspace=ws)
+    moe.synchronize(workspace=ws)
+    lens[0] = bad
+    got = attn.cache_read(cache, table, lens, count=100, workspace=ws)
+    with pytest.raises(moe.SeedlessError) as e:
+        moe.synchronize(workspace=ws)
+    assert e.value.status == 11
+    for a, r in zip(got, want):
+        assert torch.equal(a[1], r[1])
+        assert torch.equal(a[0], torch.zeros_like(r[0]) if bad < 0 else r[0])  # (the pages that are there)
