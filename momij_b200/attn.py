@@ -154,6 +154,11 @@ def attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens: 
     Token rows of ``q`` and ``out`` may be strided.  Without a workspace the call makes
     one of its own, and nothing reports a page or length out of range."""
     def call():
+        if workspace is None:  # (with one, the call itself looks at q)
+            if not isinstance(q, torch.Tensor):
+                raise TypeError("q is a tensor")
+            if q.dim() != 3:
+                raise ValueError("q is [T, Hq, D]")
         ws = new_workspace(q.shape[0], q.shape[1], device=q.device) if workspace is None else workspace
         return _ops.attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lens, scale, window, cu_q, max_q, out, ws)
     return _on(stream, call)

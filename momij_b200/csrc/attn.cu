@@ -602,8 +602,8 @@ extern "C" int momij_attention(const void* q, long long ldq, void* out, long lon
     if (T < 0 || B < 0 || n_pages < 0 || table_cols < 0 || max_q < 0 || window < 0) return MOMIJ_ERR_INVALID_ARGUMENT;
     if (dtype != MOMIJ_DTYPE_BF16 && dtype != MOMIJ_DTYPE_F16) return MOMIJ_ERR_INVALID_ARGUMENT;
     if (Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || (D != 64 && D != 128) || table_cols > (1 << 24)) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
-    if (T == 0 || B == 0) return MOMIJ_OK;
-    if (!cu_q && T % B != 0) return MOMIJ_ERR_INVALID_ARGUMENT;
+    if (T == 0) return MOMIJ_OK;
+    if (B == 0 || (!cu_q && T % B != 0)) return MOMIJ_ERR_INVALID_ARGUMENT;  // (rows of no sequence)
     if (!q || !out || !k_codes || !v_codes || !k_scales || !v_scales || !block_table || !lens || !workspace)
         return MOMIJ_ERR_INVALID_ARGUMENT;
     if (ldq < (long long)Hq * D || ldo < (long long)Hq * D || ldo % 4 != 0 || !host_aligned(q, 2) || !host_aligned(out, 8) ||

@@ -75,6 +75,11 @@ int int32(PyObject* o, const char* name) {
     if (v < -2147483647LL || v > 2147483647LL) throw ValueErr(std::string(name) + " is out of range");
     return (int)v;
 }
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw python_error();
+    return v != 0;
+}
 double real(PyObject* o) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw python_error();
@@ -204,7 +209,7 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
         }
         check(F.append(qkv.data_ptr(), T > 1 ? qkv.stride(0) : width, q.data_ptr(), ptr(qw), ptr(kw), (float)real(o[10]),
                        rope ? rope->const_data_ptr<float>() : nullptr, rope ? dim32(rope->size(0)) : 0, rope ? dim32(rope->size(1)) : 0,
-                       PyObject_IsTrue(o[12]), c.k->data_ptr<uint8_t>(), c.v->data_ptr<uint8_t>(), c.ks->data_ptr<float>(),
+                       truth(o[12]), c.k->data_ptr<uint8_t>(), c.v->data_ptr<uint8_t>(), c.ks->data_ptr<float>(),
                        c.vs->data_ptr<float>(), c.pages, table_of(table, B), dim32(table.size(1)), ints(&lens, "lens", B),
                        ints(cu, "cu_q", B + 1), dim32(T), dim32(B), int32(o[14], "max_q"), Hq, c.Hkv, c.D, dt, ptr(ws),
                        ws ? ws->nbytes() : 0, stream_of(dev)),
@@ -221,7 +226,7 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const Tensor &table = need(o[4], "block_table"), &lens = need(o[5], "lens");
         const Tensor *first = opt(o[6], "first"), *ws = workspace(o[9]);
         const int dev = on_current({c.k, c.v, c.ks, c.vs, &table, &lens, first, ws});
-        const int cnt = int32(o[7], "count"), f16 = PyObject_IsTrue(o[8]);
+        const int cnt = int32(o[7], "count"), f16 = truth(o[8]);
         value(lens.dim() == 1 && cnt >= 0, "lens is [B], count not negative");
         const int64_t B = lens.size(0);
         const at::ScalarType dt = f16 ? at::kHalf : at::kBFloat16;

@@ -623,8 +623,8 @@ extern "C" int momij_qk_norm_rope_append(const void* qkv, long long ld, void* q_
     if (dtype != MOMIJ_DTYPE_BF16 && dtype != MOMIJ_DTYPE_F16) return MOMIJ_ERR_INVALID_ARGUMENT;
     if (Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || (D != 64 && D != 128) || rot < 0 || rot > D || rot % 16 != 0 || table_cols > (1 << 24))
         return MOMIJ_ERR_UNSUPPORTED_SHAPE;
-    if (T == 0 || B == 0) return MOMIJ_OK;
-    if (!cu_q && T % B != 0) return MOMIJ_ERR_INVALID_ARGUMENT;
+    if (T == 0) return MOMIJ_OK;
+    if (B == 0 || (!cu_q && T % B != 0)) return MOMIJ_ERR_INVALID_ARGUMENT;  // (rows of no sequence)
     if (!qkv || !q_out || !k_codes || !v_codes || !k_scales || !v_scales || !block_table || !lens || (rot && !rope))
         return MOMIJ_ERR_INVALID_ARGUMENT;
     if (ld < (long long)(Hq + 2 * Hkv) * D || ld % 8 != 0 || !host_aligned(qkv, 16) || !host_aligned(q_out, 16) || !host_aligned(rope, 16) ||

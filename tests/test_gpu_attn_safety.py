@@ -319,3 +319,20 @@ def test_cache_read_reports_lengths_out_of_range(bad):
     for a, r in zip(got, want):
         assert torch.equal(a[1], r[1])
         assert torch.equal(a[0], torch.zeros_like(r[0]) if bad < 0 else r[0])  # (the pages that are there)
+
+
+def test_refusals_of_odd_arguments():
+    q, cache, table, lens = device_args(1, 2, 64, 4, 2, 64, "bf16")
+    x = torch.zeros(2, 8 * 64, dtype=q.dtype, device="cuda")
+    ws = attn.new_workspace(2, 4)
+    for bad, err in ((None, TypeError), (3, TypeError), (q[0], ValueError), (q.cpu(), ValueError)):
+        for kw in ({}, dict(workspace=ws)):
+            with pytest.raises(err):
+                attn.attention(bad, cache, table, lens, **kw)
+    with pytest.raises(RuntimeError):  # a truth value that there is not
+        attn.qk_norm_rope_append(x, cache, table, lens, n_heads=4, interleaved=torch.zeros(2, device="cuda"))
+    for call in (lambda: attn.attention(q, cache, table[:0], lens[:0], workspace=ws),  # rows of no sequence
+                 lambda: attn.qk_norm_rope_append(x, cache, table[:0], lens[:0], n_heads=4)):
+        with pytest.raises(moe.SeedlessError) as e:
+            call()
+        assert e.value.status == moe.INVALID_ARGUMENT
