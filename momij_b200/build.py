@@ -60,6 +60,18 @@ def _compile(src: str, verbose_ptxas: bool) -> str:
     return out
 
 
+def _bind_is_current(out: str, deps: list[str], stamp: str, made_with: str) -> bool:
+    """Whether ``out`` is newer than its sources and was built against this torch and
+    Python (``stamp`` holds what the last build used): another's headers may lay
+    tensors out differently."""
+    if not os.path.exists(out) or os.path.getmtime(out) < max(os.path.getmtime(d) for d in deps):
+        return False
+    if not os.path.exists(stamp):
+        return False
+    with open(stamp) as f:
+        return f.read() == made_with
+
+
 def _bind() -> str:
     """_momij_ops.so: the Python entry of the attn and head operators (a CPython
     module over torch's tensors; libmomij_moe.so itself needs neither)."""
@@ -69,7 +81,8 @@ def _bind() -> str:
     src = os.path.join(CSRC, "bind.cpp")
     out = os.path.join(LIB_DIR, "_momij_ops.so")
     deps = [src, os.path.join(ROOT, "include", "momij_moe.h")]
-    if os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(d) for d in deps):
+    stamp, made_with = os.path.join(OBJ, "bind.stamp"), f"{torch.__version__} {torch.version.cuda} {torch.__file__} {sys.version}"
+    if _bind_is_current(out, deps, stamp, made_with):
         return out
     inc, lib = os.path.join(os.path.dirname(torch.__file__), "include"), os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda = os.path.dirname(os.path.dirname(nvcc()))
@@ -81,6 +94,8 @@ def _bind() -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for bind.cpp:\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write(made_with)
     return out
 
 
