@@ -323,8 +323,11 @@ size_t momij_attention_workspace_size(int T, int Hq);
  * positions p - window < j <= p of the token's sequence (window 0: all), with
  * p = lens[b] - n_b + i for its i-th new token; kv head hq / (Hq / Hkv).  A row
  * that sees no position (lens[b] < n_b) gives zeros.  Rows of q and out are ldq
- * and ldo elements apart (ldo % 4 == 0).  One launch, or a second that joins what
- * blocks share (more than 16 rows per kv head, few heads); the result does not
+ * and ldo elements apart (ldo % 4 == 0).  max_q * Hq / Hkv is at most 524,288 rows
+ * (so a batch of many tokens gives its max_q), and their tiles of 128 rows times
+ * Hkv * table_cols at most 2^30; more is refused as MOMIJ_ERR_UNSUPPORTED_SHAPE.  One
+ * launch for every 4,096 sequences (or row tiles), and a second that joins what blocks
+ * share (more than 16 rows per kv head, few heads); the result does not
  * depend on scheduling.
  * Replaces: the 16-bit attention of SeedlessMetal.swift:2794-3004. */
 int momij_attention(const void* q, long long ldq, void* out, long long ldo, const uint8_t* k_codes,

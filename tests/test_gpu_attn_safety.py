@@ -336,3 +336,43 @@ def test_refusals_of_odd_arguments():
         with pytest.raises(moe.SeedlessError) as e:
             call()
         assert e.value.status == moe.INVALID_ARGUMENT
+
+
+def shared_pages(B, cols, Hkv, D, seed=0):
+    """Sequences that read pages of one small pool: (pool, table)."""
+    pool = R.random_pool(50, Hkv, D, seed)
+    return pool, torch.randint(0, 50, (B, cols), generator=torch.Generator().manual_seed(seed + 1), dtype=torch.int32)
+
+
+def test_more_sequences_than_a_launch_takes():
+    B, Hq, D = 4_100, 4, 64
+    pool, table = shared_pages(B, 2, 1, D)
+    lens = [1 + (b * 37) % 128 for b in range(B)]
+    q = torch.randn(B, Hq, D, generator=torch.Generator().manual_seed(2)).bfloat16()
+    ws = attn.new_workspace(B, Hq)
+    out = attn.attention(q.cuda(), attn.KVCache(*(t.cuda() for t in pool)), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), workspace=ws)
+    moe.synchronize(workspace=ws)
+    ref, mag, big = R.attention(q, *pool, table, lens, list(range(B + 1)))
+    assert bool(((out.cpu().double() - ref).abs() <= R.attention_bound(ref, mag, big, D, q.dtype)).all())
+
+
+def test_more_row_tiles_than_a_launch_takes():
+    """34 sequences of 128 row tiles (32 a launch); a window of one: each token's output is
+    its own value.  And a sequence of more tiles than a launch takes is refused."""
+    B, n, Hq, D = 34, 2048, 8, 64
+    pool, table = shared_pages(B, n // 64, 1, D)
+    q = torch.randn(B * n, Hq, D, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    cache = attn.KVCache(*(t.cuda() for t in pool))
+    ws = attn.new_workspace(B * n, Hq)
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    out = attn.attention(q, cache, table.cuda(), lens, window=1, workspace=ws)
+    moe.synchronize(workspace=ws)
+    want = R.values(*pool)[1].cuda()[table.long().cuda()][:, :, 0].reshape(B * n, 1, D)
+    err = (out.double() - want).abs()
+    assert bool((err <= R.attention_bound(want, want.abs(), 0.0, D, q.dtype)).all())
+    # 65,537 tokens of eight heads to a kv head: 4,097 tiles
+    big = torch.zeros(65_537, 8, D, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(moe.SeedlessError) as e:
+        attn.attention(big, cache, torch.zeros(1, 1025, dtype=torch.int32, device="cuda"),
+                       torch.tensor([65_537], dtype=torch.int32, device="cuda"), workspace=ws)
+    assert e.value.status == moe.UNSUPPORTED_SHAPE
