@@ -17,16 +17,16 @@
 // power of two, which holds bf16's 8 bits exactly.
 //
 // Work.  A cache read once is all that a decode step needs, so the heads of a
-// group and the drafted tokens share it: a row block is 8 or 16 (token,
-// head) rows of one sequence and one kv head, multiplied by mma.sync m16n8k16
-// with the cache's codes as the 16-row operand (tokens for the scores,
+// group and the drafted tokens share it: the up to 16 (token, head) rows of one
+// sequence and kv head (attn_prefill.cu takes more), multiplied by mma.sync
+// m16n8k16 with the cache's codes as the 16-row operand (tokens for the scores,
 // dimensions for the outputs) and the rows as its 8 columns: a decode step's
 // few rows waste little, every code is converted once, and the outputs take
 // 32 registers per 8 rows (tcgen05's 128 rows would be mostly empty).  The
 // weights turn from the first product's result into the second's operand by
 // an 8x8 transposition between lanes (movmatrix).
 //
-// The (row block, head, page) triples of all sequences form one line that is
+// The (sequence, head, page) triples of all sequences form one line that is
 // cut into equal shares, one per block, so that ragged batches load every SM
 // alike; a block's warps take half pages in turn, each through its own ring of
 // cp.async stages (no barrier in the loop), and join their results at the end.
@@ -41,10 +41,10 @@
 namespace momij {
 namespace {
 
-constexpr int kMaxSeg = 4096;   // row blocks per launch (their prefix sums live in shared memory)
+constexpr int kMaxSeg = 4096;   // sequences per launch (their prefix sums live in shared memory)
 constexpr int kMinPages = 4;    // pages per block at least, unless the segments are shorter
 constexpr int kStartPages = 10, kJoinPages = 8;  // what a piece's start and a join cost: about 4 and 3 us against 0.37 a page
-constexpr int kMaxRows = 16;    // rows of a row block at most
+constexpr int kMaxRows = 16;    // rows of a sequence and kv head at most
 constexpr int kWarps = 12, kThreads = kWarps * 32;
 constexpr int kStages = 2;      // of a warp's ring
 
@@ -67,21 +67,18 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     return r;
 }
 
-// Pages [lo, hi) that the rows of one row block see.
+// Pages [lo, hi) that a sequence's rows see.
 struct Span {
     int lo, hi, rows;
 };
-__device__ __forceinline__ Span span_of(const AttnArgs& a, const AttnSeq& s, int rb, int RB) {
+__device__ __forceinline__ Span span_of(const AttnArgs& a, const AttnSeq& s) {
     Span p{0, 0, 0};
     if (!s.ok) return p;
-    const int r0 = rb * RB, r1 = min(r0 + RB, s.n * a.G);
-    if (r0 >= r1) return p;
-    p.rows = r1 - r0;
-    const int top = s.past + (r1 - 1) / a.G + 1;  // keys below it
-    if (top <= 0) return p;
-    const int low = a.window > 0 ? max(0, s.past + r0 / a.G - a.window + 1) : 0;
+    p.rows = s.n * a.G;
+    if (p.rows == 0 || s.len == 0) return p;
+    const int low = a.window > 0 ? max(0, s.past - a.window + 1) : 0;
     p.lo = low / kPage;
-    p.hi = (top + kPage - 1) / kPage;
+    p.hi = (s.len + kPage - 1) / kPage;
     return p;
 }
 
@@ -108,14 +105,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
     const int stopped = __syncthreads_or(tid == 0 && cache_stopped(a.ws, a.stop, a.stop_step));
 
     // ---- prefix sums of the segments' pages, and the segments that have any ---
-    const int nseg = a.nb * a.nrb, per = (nseg + kThreads - 1) / kThreads;
+    const int nseg = a.nb, per = (nseg + kThreads - 1) / kThreads;
     int sum = 0, full = 0, most = 0;
     for (int i = 0; i < per; ++i) {
         const int sg = tid * per + i;
         if (sg < nseg) {
-            const AttnSeq s = attn_sequence(a, a.b0 + sg / a.nrb);
-            const Span p = span_of(a, s, sg % a.nrb, RB);
-            if (!s.ok && sg % a.nrb == 0) cache_error(a.ws, MOMIJ_ERR_PAGE);
+            const AttnSeq s = attn_sequence(a, a.b0 + sg);
+            const Span p = span_of(a, s);
+            if (!s.ok) cache_error(a.ws, MOMIJ_ERR_PAGE);
             sum += p.hi - p.lo;
             full += p.hi > p.lo;
             most = max(most, p.hi - p.lo);
@@ -153,10 +150,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
     if (nfull < nseg && !stopped)
         for (int sg = blockIdx.x; sg < nseg; sg += gridDim.x)
             if (s_pref[sg + 1] == s_pref[sg]) {
-                const AttnSeq s = attn_sequence(a, a.b0 + sg / a.nrb);
-                const Span p = span_of(a, s, sg % a.nrb, RB);
+                const AttnSeq s = attn_sequence(a, a.b0 + sg);
+                const Span p = span_of(a, s);
                 for (int i = tid; i < p.rows * a.Hkv * D; i += kThreads) {
-                    const int d = i % D, h = i / D % a.Hkv, r = i / D / a.Hkv + (sg % a.nrb) * RB;
+                    const int d = i % D, h = i / D % a.Hkv, r = i / D / a.Hkv;
                     a.out[(s.t0 + r / a.G) * a.ldo + (h * a.G + r % a.G) * D + d] = 0;
                 }
             }
@@ -171,9 +168,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
     int u = u0;
     while (u < u1) {
         while (s_pref[seg + 1] * a.Hkv <= u) ++seg;
-        const int b = a.b0 + seg / a.nrb, row0 = (seg % a.nrb) * RB;
+        const int b = a.b0 + seg;
         const AttnSeq sq = attn_sequence(a, b);
-        const Span span = span_of(a, sq, seg % a.nrb, RB);
+        const Span span = span_of(a, sq);
         const int np = span.hi - span.lo;
         const int sbase = s_pref[seg] * a.Hkv;
         const int h = (u - sbase) / np;
@@ -191,8 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
 
         // ---- this warp's half pages -------------------------------------------
         const int n_items = 2 * (pb - pa);
-        const int keys_hi = sq.past + (row0 + span.rows - 1) / a.G + 1;
-        const int keys_lo = a.window > 0 ? max(0, sq.past + row0 / a.G - a.window + 1) : 0;
+        const int keys_hi = sq.len, keys_lo = a.window > 0 ? max(0, sq.past - a.window + 1) : 0;
         unsigned char* ring = smem + warp * (kStages * kStage);
         const uint32_t ring32 = smem_u32(ring);
         // A lane's 16 bytes of a copy of 512: K rows of 128 bytes swap their
@@ -241,10 +237,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
         uint32_t qf[NB][KS][2];
         float fac[NB][2], shift[NB][2];  // per row 2c, 2c + 1: factor of the scores, and what the codes' offset adds to them
         auto load_q = [&](int nb, uint32_t (&f)[KS][2]) -> float2 {
-            const int r = 8 * nb + g, row = row0 + r;
+            const int r = 8 * nb + g;
             float e[D / 64][16];
             uint32_t top = 0;
-            const uint16_t* src = a.q + (sq.t0 + row / a.G) * a.ldq + (h * a.G + row % a.G) * D + 16 * c;
+            const uint16_t* src = a.q + (sq.t0 + r / a.G) * a.ldq + (h * a.G + r % a.G) * D + 16 * c;
 #pragma unroll
             for (int i = 0; i < D / 64; ++i) {
                 uint32_t w[8];
@@ -305,9 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
 #pragma unroll
             for (int k = 0; k < MD; ++k) o[nb][k][0] = o[nb][k][1] = o[nb][k][2] = o[nb][k][3] = 0.f;
         }
-        // keys that every row of the block sees
-        const int all_hi = sq.past + row0 / a.G + 1;
-        const int all_lo = a.window > 0 ? sq.past + (row0 + span.rows - 1) / a.G - a.window + 1 : 0;
+        // keys that every row sees
+        const int all_hi = sq.past + 1, all_lo = a.window > 0 ? sq.len - a.window : 0;
 
         int stage = 0;
         for (int it = 0; warp + kWarps * it < n_items; ++it) {
@@ -368,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
                 if (!inside) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int r = 8 * nb + 2 * c + e, pos = sq.past + (row0 + r) / a.G;
+                        const int r = 8 * nb + 2 * c + e, pos = sq.past + r / a.G;
                         const int khi = r < span.rows ? pos + 1 : 0, klo = a.window > 0 ? pos - a.window + 1 : 0;
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
@@ -465,12 +460,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs a) {
         float* part = a.parts + (long long)(2 * blockIdx.x + (u != u0)) * kPart;
         constexpr int Q4 = D / 4;
         auto finish = [&](int r, int q4, float4 v, float sum_w) {
-            const int row = row0 + r;
             const float inv = sum_w == 0.f ? 0.f : __fdividef(1.f, sum_w);
             uint2 w;
             w.x = Half<DT>::from_f(v.x * inv) | ((uint32_t)Half<DT>::from_f(v.y * inv) << 16);
             w.y = Half<DT>::from_f(v.z * inv) | ((uint32_t)Half<DT>::from_f(v.w * inv) << 16);
-            *reinterpret_cast<uint2*>(a.out + (sq.t0 + row / a.G) * a.ldo + (h * a.G + row % a.G) * D + 4 * q4) = w;
+            *reinterpret_cast<uint2*>(a.out + (sq.t0 + r / a.G) * a.ldo + (h * a.G + r % a.G) * D + 4 * q4) = w;
         };
         for (int i = tid; i < span.rows * Q4; i += kThreads) {
             const int r = i / Q4, q4 = i % Q4;
@@ -563,7 +557,7 @@ template <int DT, int D, int NB>
 int launch(const AttnArgs& a, int grid, momij_stream_t st) {
     constexpr int RB = 8 * NB;
     constexpr size_t ring = (size_t)kWarps * kStages * 64 * D, join = (size_t)kWarps * RB * (D + 4) * 4;
-    const size_t smem = (ring > join ? ring : join) + 2 * kWarps * RB * 4 + ((size_t)a.nb * a.nrb + 1) * 4;
+    const size_t smem = (ring > join ? ring : join) + 2 * kWarps * RB * 4 + ((size_t)a.nb + 1) * 4;
     static int granted[64];
     if (!host_allow_smem(attn_kernel<DT, D, NB>, smem, granted)) return MOMIJ_ERR_CUDA;
     return host_launch(attn_kernel<DT, D, NB>, dim3(grid), dim3(kThreads), smem, st, a);
@@ -650,12 +644,10 @@ extern "C" int momij_attention(const void* q, long long ldq, void* out, long lon
     const long long rows = (long long)a.longest * a.G;
     if (rows >= kPrefillRows) return attn_prefill_launch(a, D, dtype, sms, stream);
     const int rb = rows <= 8 ? 8 : 16;
-    const long long nrb = (rows + rb - 1) / rb;  // (1: more rows go to tcgen05)
-    // sequences per launch: their row blocks and units (row block, head, page) stay countable
-    const long long units = nrb * Hkv * std::max(table_cols, 1);
-    if (nrb > kMaxSeg || units > (1LL << 30)) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
-    a.nrb = (int)nrb;
-    const int per = (int)std::min<long long>(kMaxSeg / nrb, (1LL << 30) / units);
+    // sequences per launch: their units (sequence, head, page) stay countable
+    const long long units = (long long)Hkv * std::max(table_cols, 1);
+    if (units > (1LL << 30)) return MOMIJ_ERR_UNSUPPORTED_SHAPE;
+    const int per = (int)std::min<long long>(kMaxSeg, (1LL << 30) / units);
     for (int b = 0; b < B; b += per) {
         a.b0 = b;
         a.nb = std::min(per, B - b);

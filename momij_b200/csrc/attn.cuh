@@ -18,7 +18,7 @@ struct AttnArgs {
     int stop_step;       // words between the blocks' views of the stop flag
     long long ldq, ldo;
     int T, B, Hq, Hkv, G, n_pages, table_cols, window, longest;
-    int b0, nb, nrb;     // sequences of this launch, row blocks per sequence
+    int b0, nb, nrb;     // sequences of this launch; attn_prefill.cu: row tiles per sequence
     int qvec;            // q rows start on 16-byte boundaries
     int spin;
     float scale_log2;    // softmax scale * log2(e)
@@ -86,7 +86,7 @@ __device__ __forceinline__ RowScale row_scale(float top) {
     return {__uint_as_float((uint32_t)(267 - e) << 23), __uint_as_float((uint32_t)(e - 13) << 23)};
 }
 
-// How a launch's line of units (row block or tile, head, stretch of keys; heads
+// How a launch's line of units (sequence or row tile, head, stretch of keys; heads
 // inside a segment) is cut into blocks: equal shares wherever they fall, or, where
 // that costs more, `parts` blocks for each (segment, head) -- short contexts, whose
 // pieces cost more to start and to join than the longest of them takes.
