@@ -297,7 +297,7 @@ template <int DT, int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(const PrefillArgs pa, int grid, int stretch) {
     extern __shared__ int s_pref[];
     const AttnArgs& a = pa.a;
-    const int nseg = a.nb * a.nrb, lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
     const Line line = make_line<256>(a, s_pref, grid);
     int seg = blockIdx.x / a.Hkv;
     const int h = blockIdx.x - seg * a.Hkv, tiles = s_pref[seg + 1] - s_pref[seg];  // (the grid has the segments' heads)
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
     __shared__ uint32_t s_tmem;
     __shared__ float s_m[2][kTileQ], s_l[2][kTileQ];  // of even and odd pages, at the end
     __shared__ uint32_t s_top[2][kTileQ];             // q's largest magnitude in each half of a row (not s_m: the row's other thread may still read that)
-    __shared__ int s_abort, s_last;
+    __shared__ int s_abort, s_last;  // s_abort: the error that ends the block's work, from a wait that gave up or from the start
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;  // warps 0-7 softmax, 8-15 convert, 16 mma
 
     if (tid == 0) {
@@ -384,18 +384,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
         mbar_init(&b_o, 1);
         mbar_init(&b_fin, 1);
         mbar_fence_init();
-        s_abort = 0;
     }
     pdl_wait();
-    const int stopped = __syncthreads_or(tid == 0 && cache_stopped(a.ws, a.stop, a.stop_step));
+    // A block that saw the stop flag goes the way of one whose waits gave up: its MMA
+    // warp issues nothing.  (A way of its own that walked the pieces cost the other
+    // roles registers: 165 us instead of 154 for 2,048 tokens of 8,192.)
+    if (tid == 0) s_abort = cache_stopped(a.ws, a.stop, a.stop_step) ? MOMIJ_ERR_STOPPED : MOMIJ_OK;
 
     int* s_pref = reinterpret_cast<int*>(smem_raw + SM::kBytes);
     const int nseg = a.nb * a.nrb;
     const Line line = make_line<kThreads>(a, s_pref, gridDim.x);
 
     // rows that see no key at all
-    for (int sg = blockIdx.x; sg < nseg && !stopped; sg += gridDim.x)
-        if (s_pref[sg + 1] == s_pref[sg]) {
+    for (int sg = blockIdx.x; sg < nseg; sg += gridDim.x)
+        if (s_pref[sg + 1] == s_pref[sg] && s_abort == MOMIJ_OK) {
             const AttnSeq s = attn_sequence(a, a.b0 + sg / a.nrb);
             const Span p = span_of(a, s, sg % a.nrb);
             if (!s.ok && tid == 0 && sg % a.nrb == 0) cache_error(a.ws, MOMIJ_ERR_PAGE);
@@ -408,23 +410,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
     int u0, u1, seg;
     line.range(blockIdx.x, nseg, u0, u1, seg);
     if (u0 >= u1) return;
-    if (stopped) {  // its parts are left out, which whoever joins them has to know
-        for (int u = u0; u < u1;) {
-            const Piece p = piece_at(a, s_pref, u, u1, seg);
-            if (p.jb - p.ja < p.span.tiles) {
-                if (pa.defer) {
-                    float* part = a.parts + (long long)(2 * blockIdx.x + (u != u0)) * part_floats(D);
-                    if (tid < p.span.rows) part[kTileQ * D + tid] = NAN;
-                } else if (tid == 0) {
-                    int cf, cl, slot;
-                    line.sharers(seg, p.h, p.start, p.span.tiles, cf, cl, slot);
-                    arrive(a.counters, cf, cl, true);
-                }
-            }
-            u += p.jb - p.ja;
-        }
-        return;
-    }
 
     if (warp == kMmaWarp) tmem_alloc(&s_tmem, 512);
     tc_before_sync();
@@ -434,13 +419,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
     const volatile int* abort = &s_abort;
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         if (mbar_wait_bounded(bar, parity, a.spin, abort)) return true;
-        s_abort = 1;
+        if (*abort == MOMIJ_OK) s_abort = MOMIJ_ERR_TIMEOUT;
         return false;
     };
 
     if (warp >= kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
-        if (warp == kMmaWarp) {
+        if (warp == kMmaWarp && *abort == MOMIJ_OK) {
             // The whole warp walks the loop, so that addresses stay uniform; one
             // lane issues.  Descriptors advance in their low word: 16 elements of
             // a row are 32 bytes, the next 64 lie an atom further.
@@ -507,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             // nothing of this warp's may be in flight when tensor memory is freed
             commit(&b_fin);
             int zero = 0;
-            if (!mbar_wait_bounded(&b_fin, 0, max(a.spin, 1 << 20), &zero)) s_abort = 1;
+            if (!mbar_wait_bounded(&b_fin, 0, max(a.spin, 1 << 20), &zero)) s_abort = MOMIJ_ERR_TIMEOUT;
         }
     } else if (warp >= kConvWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
@@ -775,14 +760,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
             ok = __all_sync(0xffffffffu, ok && wait(&b_o, piece & 1));
             tc_after_sync();
             // ---- results: the two kinds of pages joined, half of the columns a thread -----
-            s_m[e][r] = ok ? m : NAN;  // (a maximum itself is never NaN)
+            s_m[e][r] = m;
             s_l[e][r] = l;
             bar_sync(1, 256);
             const float m0 = s_m[0][r], m1 = s_m[1][r];
             m = fmaxf(m0, m1);
             const float w0 = m0 == m ? 1.f : ex2(m0 - m), w1 = m1 == m ? 1.f : ex2(m1 - m);
             l = s_l[0][r] * w0 + s_l[1][r] * w1;
-            const bool whole = p.ja == 0 && p.jb == p.span.tiles, mine = r < rows && m0 == m0 && m1 == m1;
+            // (a row's other thread that gave up said so before the barrier)
+            const bool good = *abort == MOMIJ_OK, whole = p.ja == 0 && p.jb == p.span.tiles, mine = r < rows && (good || !whole);
             float* part = a.parts + (long long)(2 * blockIdx.x + (u != u0)) * part_floats(D);
             uint16_t* dst = a.out + (sq.t0 + tok) * a.ldo + hq * D + e * DH;
             const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
@@ -814,8 +800,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
                 }
             }
             if (!whole) {
-                if (r < rows && e == 0) {
-                    part[kTileQ * D + r] = mine ? m : NAN;
+                if (mine && e == 0) {
+                    part[kTileQ * D + r] = good ? m : NAN;
                     part[kTileQ * (D + 1) + r] = l;
                 }
                 if (!pa.defer) {
@@ -824,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
                     int cf, cl, slot;
                     line.sharers(seg, h, p.start, p.span.tiles, cf, cl, slot);
                     if (tid == 0) {
-                        s_last = arrive(a.counters, cf, cl, *abort != 0);
+                        s_last = arrive(a.counters, cf, cl, !good);
                         __threadfence();
                     }
                     bar_sync(1, 256);
@@ -840,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
     __syncthreads();
     tc_after_sync();
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
-    if (tid == 0 && s_abort) cache_error(a.ws, MOMIJ_ERR_TIMEOUT);
+    if (tid == 0 && s_abort != MOMIJ_OK) cache_error(a.ws, s_abort);
     pdl_launch_dependents();
 }
 
