@@ -21,7 +21,7 @@ def qmm4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.T
     [N, K/8] (code k of a word at bits 4k .. 4k+3) with ``scales``, ``biases`` [N, K/gs].
     Rows of ``x`` and ``out`` may be strided."""
     if stream is not None:
-        return _on(stream, lambda: qmm4(x, w, scales, biases, gs=gs, out=out))
+        return _on(stream, qmm4, x, w, scales, biases, gs=gs, out=out)
     return _ops.qmm4(x, w, scales, biases, gs, out)
 
 
@@ -35,7 +35,6 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     ``allowed`` (int32 [B, ceil(V/32)], bit v%32 of word v//32) has a zero bit.
     ``out`` may be ``logits`` itself where that is fp32."""
     if stream is not None:
-        return _on(stream, lambda: process_logits(
-            logits, history=history, cu_history=cu_history, repetition=repetition, presence=presence, frequency=frequency,
-            bias_ids=bias_ids, bias=bias, cu_bias=cu_bias, allowed=allowed, out=out))
+        return _on(stream, process_logits, logits, history=history, cu_history=cu_history, repetition=repetition, presence=presence,
+                   frequency=frequency, bias_ids=bias_ids, bias=bias, cu_bias=cu_bias, allowed=allowed, out=out)
     return _ops.logits(logits, history, cu_history, repetition, presence, frequency, bias_ids, bias, cu_bias, allowed, out)
