@@ -25,13 +25,13 @@
 // What bounds it: the launch and three dependent reads (length, page, rows) for
 // single tokens (1 token: 3 us, as much for its values); instructions for a
 // prompt's chunk.  4099 tokens of 16 + 2 x 4 heads of 128, 46 MB, with the values
-// read back, 17 MB more: 16.9 us, of which 9 are bytes.  What brought that down
+// read back, 17 MB more: 17.2 us, of which 9 are bytes.  What brought that down
 // from 55: the whole page in one block's registers (27.7), and then half the
 // instructions: packed fp32 arithmetic with registers paired so that a rotation
 // needs no moves, one lane for neighbouring rows so that V turns by byte permutes,
 // all heads of a token in one warp; the raw heads and a page's angles come
 // asynchronously through shared memory, which keeps four blocks on an SM (three:
-// 18.4; two blocks of 512 threads: 21.5).
+// 18.4; two blocks of 512 threads: 21.5); then 16.9 became 17.2 for quotients rounded once.
 #include <algorithm>
 
 #include "host.cuh"
@@ -139,6 +139,12 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
     return r;
 }
 
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // A head row lies in L = D / 8 lanes, eight elements each, as four pairs: of
 // neighbours, or with interleaved rotation (IL) of elements two apart, so that x and
 // what it turns with are the same half of two registers.
@@ -240,10 +246,24 @@ __device__ __forceinline__ void others(const uint4& raw, const F2 (&x)[4], int f
     for (int k = 0; k < 4; ++k) o[k] = IL ? x[k ^ 1] : f2(unpack<DT>(__shfl_sync(0xffffffffu, word(raw, k), from)));
 }
 
-// Codes 128 + rint(x / scale): the addition of 1.5 * 2^23 + 128 rounds to a whole
-// number (ties to even) and leaves it in the low byte; |x| / scale is at most 127 and
-// a rounding error.  (Of a page with a NaN scale the codes do not matter.)
-__device__ __forceinline__ F2 coded(F2 x, F2 inv) { return fma2(x, inv, f2(12583040.f, 12583040.f)); }
+// Codes 128 + rint(x / scale), ties to even.  Values of 16 bits meet a tie often (an
+// amax that 127 divides makes every second half a code one), so the quotient is the
+// correctly rounded one of numbers without an error: of x 127 / 128 by amax / 128 where
+// the page's scale is these rows' amax / 127, of x by the old scale where that holds.
+// A product with the reciprocal, its residual and one correction (Markstein's division)
+// round it so; the addition of 1.5 * 2^23 + 128 then leaves the whole number in the low
+// byte.  |x| / scale is at most 127.  (Of a page with a NaN scale the codes do not matter.)
+struct Coder {
+    F2 factor, minus, inv;
+    __device__ __forceinline__ Coder(float mul, float den) : factor(f2(mul, mul)), minus(f2(-den, -den)) {
+        const float r = den > 0.f ? 1.f / den : 0.f;
+        inv = f2(r, r);
+    }
+    __device__ __forceinline__ F2 operator()(F2 x) const {
+        const F2 n = mul2(x, factor), t = mul2(n, inv);
+        return add2(fma2(fma2(t, minus, n), inv, t), f2(12583040.f, 12583040.f));
+    }
+};
 __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
     return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040),
                        0x5410);
@@ -429,14 +449,16 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) append_kernel(const Ap
     }
     __syncthreads();  // (every thread has read the old scale, too)
     // The scale; infinities and NaN make it NaN, and the page reads as NaN.
-    float scale = __uint_as_float(s_top) * (1.f / 127.f);
+    const float amax = __uint_as_float(s_top);
+    float scale = amax / 127.f;
     if (scale < kMinScale) scale = 0.f;
+    const bool own = scale > had;  // the page's scale is the new rows'
     if (s_top >= 0x7f800000u || !(had <= 3.0e38f)) scale = __int_as_float(0x7fffffff);
     else scale = fmaxf(scale, had);
     const float inv = scale > 0.f ? 1.f / scale : 0.f;
     const bool grew = r0 > 0 && scale > had;  // (false for a NaN scale: its codes do not matter)
     const float ratio = had * inv;
-    const F2 inv2 = f2(inv, inv);
+    const Coder coded(own ? 127.f / 128.f : 1.f, own ? amax * (1.f / 128.f) : scale);
     if (tid == 0) *scale_at = scale;
 
     if (!is_v) {
@@ -446,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) append_kernel(const Ap
             for (int i = 0; i < R; ++i) {
                 if (p0 + i < r0 || p0 + i >= r1) continue;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[i][k] = coded(x[i][k], inv2);
+                for (int k = 0; k < 4; ++k) x[i][k] = coded(x[i][k]);
                 float e[8];
                 elements_of<IL>(x[i], e);
                 *reinterpret_cast<uint2*>(dst + (p0 + i) * D + 8 * l) =
@@ -467,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) append_kernel(const Ap
             for (int k = 0; k < 4; ++k) {
                 float2 v[R];
 #pragma unroll
-                for (int i = 0; i < R; ++i) v[i] = parts(coded(x[i][k], inv2));
+                for (int i = 0; i < R; ++i) v[i] = parts(coded(x[i][k]));
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     uint32_t* at = s_v + (8 * l + 2 * k + e) * 16 + ((p0 >> 2) ^ (l & 15));
