@@ -293,9 +293,11 @@ int momij_moe_block(void* h, const void* norm_w, float eps, const void* w_gate, 
  *   (rope fp32 [rope_rows, rot]: rot/2 cosines, then rot/2 sines; pairs
  *   (i, i + rot/2), or (2i, 2i + 1) if interleaved; rot % 16 == 0, 0: none)
  * q_out [T, Hq, D] gets the queries; keys and values become codes at positions
- * lens[b] - n_b .. lens[b] - 1.  A page's scale is amax / 127 over its tokens so
- * far; when new tokens raise it, the page's earlier tokens are recoded (rounded
- * once more).  A page that receives an infinity or NaN gets a NaN scale and
+ * lens[b] - n_b .. lens[b] - 1.  A page's scale is amax / 127 over the tokens written
+ * to it since its first row; when new tokens raise it, the page's earlier tokens are
+ * recoded: rounded once more, by at most half a code of the new scale.  Tokens taken
+ * back by a smaller length (a rejected draft) leave the scale that they brought, and
+ * that rounding, to the page's others.  A page that receives an infinity or NaN gets a NaN scale and
  * reads as NaN until its first row is written again.  Pages must not be shared
  * by sequences that append to them.  workspace may be NULL (no error report).
  * Replaces: the query/key norm with rotation (MapleFused.swift:260-325) and the
@@ -342,7 +344,7 @@ int momij_attention(const void* q, long long ldq, void* out, long long ldo, cons
  * Rows of x and y are ldx and ldy elements apart.  For few tokens: up to 32 share
  * a pass over the matrix, one launch each (fewer for K above 14,000 or so).  The call
  * has no workspace: a raised stop flag leaves y as it was, and a device-side wait that
- * gave up leaves NaN in the tile it was for.
+ * gave up leaves NaN in the tile it was for.  K is at most about 58,000.
  * Replaces: the 4-bit output head's product (SeedlessMetal.swift:2598-2716) and
  * MLX.quantizedMM of 4-bit projections (QuantProj.swift). */
 int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const void* scales, const void* biases, void* y,

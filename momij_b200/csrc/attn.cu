@@ -14,7 +14,8 @@
 // rounded to fp16 after a factor 2^15 (it cancels): 11 bits, down to 2^-29 of
 // the row's largest, and still something down to 2^-39; the sums of weights,
 // the maximum and the outputs are fp32.  q enters as fp16 scaled per row by a
-// power of two, which holds bf16's 8 bits exactly.
+// power of two: exactly, for bf16 down to 2^-30 of the row's largest element (fp16:
+// 2^-27), with an error below 2^-38 of that further down.
 //
 // Work.  A cache read once is all that a decode step needs, so the heads of a
 // group and the drafted tokens share it: the up to 16 (token, head) rows of one

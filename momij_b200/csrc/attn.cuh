@@ -157,11 +157,12 @@ struct Line {
 };
 
 // Rows (tokens times heads of a group) per sequence from which attention goes
-// to attn_prefill.cu.  Measured, us for 16 / 24 / 32 rows, attn.cu's kernel (row
-// blocks of 16 and 32) against that one's: 24 sequences of 5,003 tokens, 4 kv
-// heads of 128: 46.8 / 60.0 / 62.5 against 64.2 / 64.4 / 64.5; one of 30,000, 2 of
-// 128: 31.9 / 42.5 / 49.9 against 26.0 / 25.9 / 26.3; 4 of 2,000, 8 of 128: 20.4 /
-// 24.7 / 26.0 against 17.5 / 17.8 / 18.0.
+// to attn_prefill.cu: what attn.cu's kernel has columns for.  Measured, us for 4 / 8 /
+// 16 rows, that kernel against this one: 24 sequences of 5,003 tokens, 4 kv heads of
+// 128: 30.2 / 31.1 / 42.3 against 45.6 / 45.8 / 46.8; one of 30,000, 2 of 128: 16.6 /
+// 17.6 / 25.9 against 27.9 / 26.6 / 28.2; 4 of 2,000, 8 of 128: 11.3 / 11.6 / 15.4
+// against 16.6 / 16.7 / 17.2.  At 17 / 32 rows, of which attn.cu would read the cache
+// once for every 16, this one takes 47.2 / 48.8, 28.6 / 29.0 and 17.4 / 17.9.
 constexpr int kPrefillRows = 17;
 int attn_prefill_launch(const AttnArgs& a, int D, int dtype, int sms, momij_stream_t st);
 size_t attn_prefill_part_bytes(int sms);

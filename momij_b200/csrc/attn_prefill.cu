@@ -37,8 +37,9 @@
 // per scheduler take 1,470 cycles for their exponentials, a tile 2,150.  Two row
 // tiles per block share the conversion, but tensor memory then has no room for a
 // second S each, and scores, weights and products wait for one another (2,220
-// cycles per tile measured).  2,048 tokens of 8,192, 16 heads of 128 over 4: 152 us,
-// 788 TFLOP/s, 48 % of the measured rate (with mma.sync: 740 us).
+// cycles per tile measured).  2,048 tokens of 8,192, 16 heads of 128 over 4: 153 us
+// as a graph, 785 TFLOP/s, 48 % of the measured rate (158 called from the host; with
+// mma.sync: 740 us).
 #include <algorithm>
 
 #include "attn.cuh"

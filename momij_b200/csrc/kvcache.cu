@@ -9,10 +9,11 @@
 // or (2i, 2i+1) when interleaved) whose cosines and sines come from a table.
 // Queries are rounded to the activations' type; keys and values become codes
 // without a rounding in between.  The scale of a page and head is
-// amax / 127 over its tokens so far: an append in the middle of a page
-// keeps the old scale when the new tokens fit and otherwise recodes the page's
-// earlier tokens by old/new (each such step adds at most half a code to them;
-// a page filled one token at a time grows about ln 64 times).
+// amax / 127 over the tokens written to it since its first row: an append in the
+// middle of a page keeps the old scale when the new tokens fit and otherwise recodes
+// the page's earlier tokens by old/new (each such step adds at most half a code to
+// them; a page filled one token at a time grows about ln 64 times).  Tokens that are
+// taken back leave the scale, and the rounding that its growth brought, behind.
 //
 // A page, head and K-or-V is one block's work, so that the scale needs no
 // second launch and no exchange between blocks: the up to 64 x D new values
@@ -25,7 +26,7 @@
 // What bounds it: the launch and three dependent reads (length, page, rows) for
 // single tokens (1 token: 3 us, as much for its values); instructions for a
 // prompt's chunk.  4099 tokens of 16 + 2 x 4 heads of 128, 46 MB, with the values
-// read back, 17 MB more: 17.2 us, of which 9 are bytes.  What brought that down
+// read back, 17 MB more: 17.2 us (15.7 as a graph), of which 9 are bytes.  What brought that down
 // from 55: the whole page in one block's registers (27.7), and then half the
 // instructions: packed fp32 arithmetic with registers paired so that a rotation
 // needs no moves, one lane for neighbouring rows so that V turns by byte permutes,

@@ -15,7 +15,7 @@
 //   * Few tokens in all: one kernel, whose blocks count the history for their own
 //     stretch of 1,024 or 2,048 tokens beside the copy.
 //   * Many: every stretch reading its row's history would cost more than the
-//     copy (48 rows of 151,936 with 6,000 ids: 24.2 us in one kernel, 7.1 of them the
+//     copy (48 rows of 151,936 with 6,000 ids: 23.0 us in one kernel, 7.1 of them the
 //     copy), and a block with counts for a long stretch copies badly (few loads
 //     in flight: 29 us).  So the copy goes alone, and a second kernel, whose blocks
 //     count while the copy drains, names and rewrites; its blocks own stretches
@@ -295,8 +295,8 @@ int launch(const Args& a, int B, int sms, bool vec, momij_stream_t st) {
     const long long tokens = (long long)B * a.V;
     const bool named = a.cu_hist || a.cu_bias;
     // One kernel up to about 2.4 million tokens.  Measured with 6,000 ids a row of
-    // 151,936, us for one kernel / two: 16 rows 10.7 / 10.6, 24 rows 14.1 / 11.9, 48
-    // rows 24.2 / 18.6.
+    // 151,936, us for one kernel / two: 16 rows 10.7 / 10.6, 24 rows 14.1 / 12.0, 48
+    // rows 23.0 / 17.6.
     if (tokens < 8LL * sms * kThreads * 8) {
         const bool two = tokens >= 2LL * sms * kThreads * 4;  // 2,048 tokens a block where that leaves two blocks an SM
         if (named) return two ? launch_copy<T, 2, true>(a, B, vec, st) : launch_copy<T, 1, true>(a, B, vec, st);

@@ -14,8 +14,9 @@
 //     One AND per two codes (and one shift per eight) makes the operand; the
 //     second class's x is divided by 16 to match.
 //   * x enters as fp16 scaled by a power of two per token so that its largest
-//     magnitude lies in [2^14, 2^15): bf16's 8 significant bits always fit, so
-//     nothing is rounded but elements below 2^-38 of the token's largest.
+//     magnitude lies in [2^14, 2^15): exactly, for bf16 down to 2^-31 of the token's
+//     largest, 2^-27 where it is divided by 16 (fp16: 2^-28 and 2^-24).  Elements
+//     further down lose at most 2^-35 of the largest.
 //   * s, b, the group sums and the running sums are fp32; y is rounded once.
 //
 // What bounds it: the bytes of the matrix (K/2 + 4 K/gs per row), as long as the
@@ -24,8 +25,8 @@
 // codes and the scales and biases, which a warp copies asynchronously into a ring
 // of its own in shared memory, three batches ahead.  (With the batch after the
 // present one in registers instead: 50 us for 151,936 x 2,048 and one token; the
-// registers left room for 24 warps with 3 KB each in flight.)  That size takes 36 us,
-// 4.9 TB/s.
+// registers left room for 24 warps with 3 KB each in flight.)  That size takes 35.6 us
+// as a graph, 4.9 TB/s (39.5 called from the host).
 #include <algorithm>
 
 #include "qmm4.cuh"
@@ -375,9 +376,9 @@ extern "C" int momij_qmm4(const void* x, long long ldx, const uint32_t* w, const
     if ((long long)ntiles * share(16) <= 16LL * sms / 2 || bytes(std::min(M, 8), 16) > kSmemMost) warps = 8;
     // One token against a matrix of four batches a warp or more: two blocks of eight warps
     // an SM, which start and end their rounds apart (us for one block / two: 151,936 x
-    // 2,048 34.6 / 33.4, 60,000 x 2,048 19.2 / 17.1, 20,000 x 2,048 8.5 / 7.9; with 3.5
-    // batches, 8,192 x 4,096, 7.3 / 7.7; with seven tokens, whose x each block turns into
-    // an operand, 41.2 / 43.4).
+    // 2,048 37.0 / 35.6, 60,000 x 2,048 19.5 / 17.5, 20,000 x 2,048 8.8 / 8.0; with 3.5
+    // batches, 8,192 x 4,096, 7.8 / 7.9; with four tokens, whose x each block turns into
+    // an operand, 39.8 / 43.1, 21.6 / 20.8 and 9.9 / 10.5).
     int per_sm = 1;
     if (M == 1 && warps == kMaxWarps && (long long)ntiles * nbatch >= 4LL * kMaxWarps * sms && bytes(1, 8) <= kSmemMost / 2 - 2048) {
         warps = 8;

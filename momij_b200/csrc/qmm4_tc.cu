@@ -19,9 +19,9 @@
 // What bounds it: the eight summing warps (a chain of accumulator reads, group sums and
 // scales a batch) and close behind them the conversion (16 KB of codes and their scales
 // cost 16 x 120 instructions); a batch's bytes would come in 750 cycles.  The tensor
-// pipe is busy a tenth of the time.  151,936 x 2,048: 9 tokens 45 us, 32 tokens 54 us
-// (155 with the other kernel), 26 for the bytes alone; 20,000 x 6,400: 29 and 37 (49
-// and 152).
+// pipe is busy a tenth of the time.  151,936 x 2,048 with groups of 64: 9 tokens 47.4 us, 32
+// tokens 59.5 (61 and 158 with the other kernel), 26.7 for the bytes alone, with groups
+// of 128 44.4 and 52.7; 20,000 x 6,400: 29.6 and 42.2 (52 and 155), 28.2 and 36.0.
 // What brought it there: partial sums sent asynchronously and finished by warps of their
 // own (79 us; a releasing arrival per warp costs a microsecond a tile), two sets of
 // converting warps that take batches in turn (51.6), packed sums, scales fetched by the
@@ -611,8 +611,8 @@ int tokens_per_pass(const Qmm4Call& c) {
 
 // Above 16 tokens, or where x has more than 16,384 elements (the other kernel's blocks
 // each turn all of it into an operand, and its products cost one instruction per 16 x 8
-// results): 9 x 151,936 x 2,048 47 us here, 54 there; 8 x the same 47 and 41; 8 x 4,096
-// x 4,096 9.6 and 14.5; 2 x 300 x 8,192 8.7 and 9.4; 12 x 8,000 x 1,024 8.1 and 6.9.
+// results): 9 x 151,936 x 2,048 47.4 us here, 61.5 there; 8 x the same 47.4 and 43.9; 8 x
+// 4,096 x 4,096 9.6 and 14.3; 2 x 300 x 8,192 9.0 and 9.1; 12 x 8,000 x 1,024 7.8 and 6.7.
 bool qmm4_tc_takes(const Qmm4Call& c) {
     return (c.M > 16 || (c.M > 1 && (long long)c.M * c.K > 16384)) && c.N >= kRows && c.K >= kCols && tokens_per_pass(c) > 0 && host_tensor_map_encoder();
 }
