@@ -38,6 +38,7 @@
 
 #include "attn.cuh"
 #include "host.cuh"
+#include "pack.cuh"
 
 namespace momij {
 namespace {
@@ -49,18 +50,6 @@ constexpr int kMaxRows = 16;    // rows of a sequence and kv head at most
 constexpr int kWarps = 12, kThreads = kWarps * 32;
 constexpr int kStages = 2;      // of a warp's ring
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 // Transposes an 8x8 matrix of 16-bit values held as row g, columns 2c, 2c + 1.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t r;

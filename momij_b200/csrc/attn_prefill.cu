@@ -44,6 +44,7 @@
 
 #include "attn.cuh"
 #include "host.cuh"
+#include "pack.cuh"
 #include "tc.cuh"
 
 namespace momij {
@@ -110,31 +111,6 @@ __device__ __forceinline__ Piece piece_at(const AttnArgs& a, const int* pref, in
 // Floats of a partial result: O [128][D], maxima (NaN: the row was left out), sums.
 __host__ __device__ constexpr int part_floats(int D) { return kTileQ * (D + 2); }
 
-__device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr) {  // K-major, 128-byte swizzle, 8-row groups 1024 B apart
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
-// kind::f16, fp16 operands, fp32 accumulator, M = 128, N = n.
-__host__ __device__ constexpr uint32_t idesc_f16(int n) {
-    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accum));
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accum));
-}
-__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 template <int DT>
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     if (DT == MOMIJ_DTYPE_F16) return f16x2(lo, hi);
@@ -142,33 +118,6 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Two fp32 lanes in one 64-bit register (fma.rn.f32x2, add.rn.f32x2).
-__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ bool elect_one() {
-    uint32_t r;
-    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
-    return r != 0;
-}
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -737,21 +686,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(const Prefill
                     }
                 }
                 const float off = lv + (7.f - (m == -INFINITY ? 0.f : m));
-                const uint64_t al2 = f32x2(al, al), off2 = f32x2(off, off);
+                const uint64_t al2 = f2(al, al), off2 = f2(off, off);
                 uint64_t sum2[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        const float2 x = unpack2(fma2(f32x2(s[32 * c + i], s[32 * c + i + 1]), al2, off2));
+                        const float2 x = parts_of(fma2(f2(s[32 * c + i], s[32 * c + i + 1]), al2, off2));
                         const float y0 = ex2(x.x), y1 = ex2(x.y);
-                        sum2[(i >> 1) & 1] = add2(sum2[(i >> 1) & 1], f32x2(y0, y1));
+                        sum2[(i >> 1) & 1] = add2(sum2[(i >> 1) & 1], f2(y0, y1));
                         p[i >> 1] = f16x2(y0, y1);
                     }
                     tmem_st16(ts + 16 * c, p);
                 }
-                const float2 u0 = unpack2(sum2[0]), u1 = unpack2(sum2[1]);
+                const float2 u0 = parts_of(sum2[0]), u1 = parts_of(sum2[1]);
                 const float sum = (u0.x + u0.y) + (u1.x + u1.y);
                 l += sum == 0.f ? 0.f : sum * iv;  // a row that sees nothing of a page takes nothing of its scale either
                 tmem_st_wait();

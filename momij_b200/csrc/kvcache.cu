@@ -37,6 +37,7 @@
 
 #include "host.cuh"
 #include "kvcache.cuh"
+#include "pack.cuh"
 
 namespace momij {
 namespace {
@@ -116,36 +117,6 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// Packed fp32 arithmetic: two lanes of a 64-bit register, half the instructions.
-using F2 = uint64_t;
-__device__ __forceinline__ F2 f2(float lo, float hi) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ F2 f2(float2 v) { return f2(v.x, v.y); }
-__device__ __forceinline__ float2 parts(F2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 // A head row lies in L = D / 8 lanes, eight elements each, as four pairs: of
 // neighbours, or with interleaved rotation (IL) of elements two apart, so that x and
 // what it turns with are the same half of two registers.
@@ -162,7 +133,7 @@ template <bool IL>
 __device__ __forceinline__ void elements_of(const F2 (&x)[4], float (&e)[8]) {
 #pragma unroll
     for (int k = 0; k < 4; k += 2) {
-        const float2 a = parts(x[k]), b = parts(x[k + 1]);
+        const float2 a = parts_of(x[k]), b = parts_of(x[k + 1]);
         e[2 * k] = a.x;
         e[2 * k + 1] = IL ? b.x : a.y;
         e[2 * k + 2] = IL ? a.y : b.x;
@@ -234,7 +205,7 @@ __device__ __forceinline__ float inverse_rms(const F2 (&x)[4], float eps) {
     F2 q = mul2(x[0], x[0]);
 #pragma unroll
     for (int i = 1; i < 4; ++i) q = fma2(x[i], x[i], q);
-    const float2 s = parts(q);
+    const float2 s = parts_of(q);
     float ss = s.x + s.y;
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -271,7 +242,7 @@ __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d
 }
 // The largest magnitude; NaN if one is.
 __device__ __forceinline__ float top_of(float m, F2 x) {
-    const float2 v = parts(x);
+    const float2 v = parts_of(x);
     asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v.x)), "f"(fabsf(v.y)));
     return m;
 }
@@ -490,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) append_kernel(const Ap
             for (int k = 0; k < 4; ++k) {
                 float2 v[R];
 #pragma unroll
-                for (int i = 0; i < R; ++i) v[i] = parts(coded(x[i][k]));
+                for (int i = 0; i < R; ++i) v[i] = parts_of(coded(x[i][k]));
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     uint32_t* at = s_v + (8 * l + 2 * k + e) * 16 + ((p0 >> 2) ^ (l & 15));
@@ -621,7 +592,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
                 const uint32_t w = c[i][k >> 1];
                 const float a0 = __uint_as_float(__byte_perm(w, 0x4b000000u, k & 1 ? 0x7442 : 0x7440)) - 8388736.f;
                 const float a1 = __uint_as_float(__byte_perm(w, 0x4b000000u, k & 1 ? 0x7443 : 0x7441)) - 8388736.f;
-                const float2 v = parts(mul2(f2(a0, a1), scale2));
+                const float2 v = parts_of(mul2(f2(a0, a1), scale2));
                 y[k] = pack<DT>(v.x, v.y);
             }
             o = make_uint4(y[0], y[1], y[2], y[3]);

@@ -56,13 +56,6 @@ struct Args {
     int pitch;                   // bytes per token of the x operand
 };
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // ONE: a pass of a single token, which is column 0.  VEC: a batch's scales of a
 // row are one aligned copy; otherwise they are read where they are used.
 template <int DT, int NT, int GS, bool VEC, bool ONE>

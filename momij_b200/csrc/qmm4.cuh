@@ -3,6 +3,7 @@
 #pragma once
 
 #include "host.cuh"
+#include "pack.cuh"
 
 namespace momij {
 
@@ -16,15 +17,10 @@ struct Qmm4Call {
     int M, N, K, gs, dtype;
 };
 
-__device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 // Two results rounded to the activations' type, in one word.
 template <int DT>
 __device__ __forceinline__ uint32_t rounded2(float lo, float hi) {
-    if (DT == MOMIJ_DTYPE_F16) return f16x2_of(lo, hi);
+    if (DT == MOMIJ_DTYPE_F16) return f16x2(lo, hi);
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
@@ -74,7 +70,7 @@ __device__ __forceinline__ uint4 qmm4_operand(const uint4& v, float f, float& su
     sum = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) sum += e[q];
-    return make_uint4(f16x2_of(e[0], e[4]), f16x2_of(e[1] * 0.0625f, e[5] * 0.0625f), f16x2_of(e[2], e[6]), f16x2_of(e[3] * 0.0625f, e[7] * 0.0625f));
+    return make_uint4(f16x2(e[0], e[4]), f16x2(e[1] * 0.0625f, e[5] * 0.0625f), f16x2(e[2], e[6]), f16x2(e[3] * 0.0625f, e[7] * 0.0625f));
 }
 constexpr float kQmm4Unit = 5.9604644775390625e-08f;  // 2^-24, the unit of the codes' products
 

@@ -54,24 +54,6 @@ struct TcArgs {
     int mt, N, K, xvec, svec, stages, spin, tiles, nbatch, cap;  // cap: batches of x that a block has room for
 };
 
-__device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr) {  // K-major, 128-byte swizzle, 8-row groups 1024 B apart
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
-// kind::f16, fp16 operands, fp32 accumulator, M = 128, N = n.
-__host__ __device__ constexpr uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accum));
-}
-__device__ __forceinline__ bool elect_one() {
-    uint32_t p;
-    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
-    return p != 0;
-}
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld8_nowait(uint32_t taddr, uint32_t (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
@@ -80,23 +62,7 @@ __device__ __forceinline__ void tmem_ld8_nowait(uint32_t taddr, uint32_t (&v)[8]
 __device__ __forceinline__ void tmem_ld_nowait(uint32_t taddr, uint32_t (&v)[8]) { tmem_ld8_nowait(taddr, v); }
 __device__ __forceinline__ void tmem_ld_nowait(uint32_t taddr, uint32_t (&v)[16]) { tmem_ld16_nowait(taddr, v); }
 
-// Packed fp32 arithmetic.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
 __device__ __forceinline__ float half_pair(uint64_t v, int hi) { return __uint_as_float((uint32_t)(hi ? v >> 32 : v)); }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 
 // ---- cluster ---------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -455,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) qmm4_tc_kernel(const __grid_const
                     tmem_ld_nowait(lanes + u * DSTEP + g * NT, d);
                     const float s = half_of<DT>(sb[g], 0), b = half_of<DT>(sb[g], 1);
                     const float* xs = sums + (j * GPB + g) * NT;
-                    const uint64_t s2 = pair(s, s), b2 = pair(b, b);
+                    const uint64_t s2 = f2(s, s), b2 = f2(b, b);
                     tmem_ld_wait();
                     settle(d);
                     if (g + 1 == GPB) {
@@ -466,8 +432,8 @@ __global__ void __launch_bounds__(kThreads, 1) qmm4_tc_kernel(const __grid_const
 #pragma unroll
                     for (int i = 0; i < NH; i += 4) {
                         const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(xs + i);
-                        acc[i / 2] = fma2(b2, x.x, fma2(s2, pair(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), acc[i / 2]));
-                        acc[i / 2 + 1] = fma2(b2, x.y, fma2(s2, pair(__uint_as_float(d[i + 2]), __uint_as_float(d[i + 3])), acc[i / 2 + 1]));
+                        acc[i / 2] = fma2(b2, x.x, fma2(s2, f2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), acc[i / 2]));
+                        acc[i / 2 + 1] = fma2(b2, x.y, fma2(s2, f2(__uint_as_float(d[i + 2]), __uint_as_float(d[i + 3])), acc[i / 2 + 1]));
                     }
                 }
             }
@@ -476,8 +442,8 @@ __global__ void __launch_bounds__(kThreads, 1) qmm4_tc_kernel(const __grid_const
 #pragma unroll
             for (int i = 0; i < NH; i += 2) {
                 const float4 f = *reinterpret_cast<const float4*>(s_fac + half * NH + i);  // of two tokens
-                acc[i / 2] = mul2(mul2(acc[i / 2], pair(f.x, f.z)), pair(f.y, f.w));
-                if (!ok) acc[i / 2] = pair(NAN, NAN);
+                acc[i / 2] = mul2(mul2(acc[i / 2], f2(f.x, f.z)), f2(f.y, f.w));
+                if (!ok) acc[i / 2] = f2(NAN, NAN);
             }
             if (S == 1) {
                 const int row = t * kRows + r, most = row < a.N ? a.mt - half * NH : 0;
