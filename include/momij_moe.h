@@ -85,7 +85,8 @@ int momij_set_stop_flag(const int32_t* device_flag);
 /* For testing what a flag raised in the middle of a launch leaves behind: block i
  * of the kernels of momij_qk_norm_rope_append, momij_cache_read and
  * momij_attention reads word i * words of the stop flag (0, the default: all read
- * the same word).  Process-wide; applies to calls enqueued afterwards. */
+ * the same word; else the flag has one for every block of their launches).
+ * Process-wide; applies to calls enqueued afterwards. */
 int momij_set_stop_step(int words);
 
 /* Bound of the device-side waits (polls of an mbarrier or of the grid
